@@ -15,6 +15,8 @@ GAME_C4, GAME_TTT, GAME_NBTTT = 0, 1, 2
 EVAL_UNIFORM, EVAL_HASH, EVAL_CNN, EVAL_HOST, EVAL_ROLLOUT, EVAL_ROLLOUT_HASH = 0, 1, 2, 3, 4, 5
 FLIP_NEVER, FLIP_STREAM, FLIP_RANDOM = 0, 1, 2
 MOVE_FIRST_MAX, MOVE_SAMPLE = 0, 1
+F32, F16, BF16 = 0, 1, 2
+ACTS = {"none": 0, "relu": 1, "silu": 2}
 K3_KINDS = {None: 0, "default": 0, "wino": 1, "split": 2, "direct": 3}
 GAME_IDS = {"Connect4": GAME_C4, "TTT": GAME_TTT, "NBTTT": GAME_NBTTT}
 
@@ -37,6 +39,11 @@ class az_config(C.Structure):
 class az_stats(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("playouts", "levels", "leaf_evals", "terminal_hits", "children",
                                          "nodes_used", "games_finished", "plies", "rollout_plies", "cache_hits")]
+
+
+class az_muon_item(C.Structure):
+    _fields_ = [("w_dev", C.c_void_p), ("g_dev", C.c_void_p), ("m_dev", C.c_void_p), ("rows", C.c_int64),
+                ("cols", C.c_int64)]
 
 
 _P = C.POINTER
@@ -92,6 +99,19 @@ SIGNATURES = {
     "az_net_set_kernel": (C.c_int, [_vp, C.c_int]),
     "az_net_get_kernel": (C.c_int, [_vp]),
     "az_net_forward_dev": (C.c_int, [_vp, _i64, _vp, _vp, _vp]),
+    "az_i8_quantize_dev": (C.c_int, [C.c_int, C.c_int, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _vp]),
+    "az_i8_matmul_ws": (C.c_size_t, [_i64, _i64, _i64]),
+    "az_i8_matmul_dev": (C.c_int, [C.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, C.c_int,
+                                   C.c_int, _vp, _i64, _vp, C.c_size_t, _vp]),
+    "az_i8_linear_ws": (C.c_size_t, [_i64, _i64, _i64]),
+    "az_i8_linear_dev": (C.c_int, [C.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, C.c_int, C.c_int,
+                                   _vp, _i64, _vp, C.c_size_t, _vp]),
+    "az_orthogonalize_ws": (C.c_size_t, [_i64, _i64, _i64]),
+    "az_orthogonalize_dev": (C.c_int, [C.c_int, C.c_int, _i64, _i64, _i64, _vp, _vp, C.c_int, _P(_dbl), _dbl, _vp,
+                                       C.c_size_t, _vp]),
+    "az_muon_step_ws": (C.c_size_t, [_P(az_muon_item), _i64]),
+    "az_muon_step_dev": (C.c_int, [C.c_int, C.c_int, _P(az_muon_item), _i64, _dbl, _dbl, C.c_int, _dbl, C.c_int, _P(_dbl),
+                                   _dbl, _vp, C.c_size_t, _vp]),
     "az_set_root_children": (C.c_int, [_vp, _vp, _vp, _vp]),
     "az_puct_batch": (C.c_int, [C.c_int, _dbl, _i32, _i64, _vp, _vp, _vp, _vp, _vp]),
 }

@@ -1,0 +1,89 @@
+// az_ops.hpp -- what the operators on caller-owned device tensors share (az_int8.hip, az_ortho.hip): element types, the
+// device of a call, and the byte geometry of their matrix tiles.
+#pragma once
+#include "az_internal.hpp"
+
+namespace az {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+// rounds to nearest, ties to even, as every conversion to 16 bits here
+__device__ inline float to_f32(float v) { return v; }
+__device__ inline float to_f32(f16 v) { return (float)v; }
+__device__ inline float to_f32(bf16 v) { return (float)v; }
+template <class T>
+__device__ inline T from_f32(float v) {
+    return (T)v;
+}
+
+inline size_t dtype_size(int dtype) { return dtype == AZ_F32 ? 4 : 2; }
+inline bool dtype_ok(int dtype) { return dtype == AZ_F32 || dtype == AZ_F16 || dtype == AZ_BF16; }
+
+#define AZ_DISPATCH_DTYPE(dtype, ...)                         \
+    switch (dtype) {                                          \
+        case AZ_F32: { using T = float; __VA_ARGS__; } break; \
+        case AZ_F16: { using T = f16; __VA_ARGS__; } break;   \
+        default: { using T = bf16; __VA_ARGS__; } break;      \
+    }
+
+// Makes `device` current for one call and puts the caller's device back at its end (a caller's other work, torch's
+// first of all, goes by the current device).
+struct DeviceScope {
+    int before = -1, rc = AZ_OK;
+    explicit DeviceScope(int device) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
+            (void)hipGetLastError();
+            set_error("no usable HIP device: libazamd has no CPU path");
+            rc = AZ_ERR_NO_DEVICE;
+            return;
+        }
+        if (device < 0 || device >= n) {
+            set_error("device ordinal out of range");
+            rc = AZ_ERR_ARG;
+            return;
+        }
+        int cur = -1;
+        if (hipGetDevice(&cur) == hipSuccess && cur == device) return;
+        if (hipSetDevice(device) != hipSuccess) {
+            (void)hipGetLastError();
+            set_error("hipSetDevice failed");
+            rc = AZ_ERR_HIP;
+            return;
+        }
+        before = cur;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+inline int launch_status(const char* fn) {
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) return AZ_OK;
+    set_error(std::string(fn) + ": " + hipGetErrorString(e));
+    return AZ_ERR_HIP;
+}
+inline int refuse(const char* what) {
+    set_error(what);
+    return AZ_ERR_ARG;
+}
+
+// ---- matrix tiles ----------------------------------------------------------------------------------------------------
+// Both products (int8, and fp32 as split fp16) read their operands along the reduction axis, 128 bytes of a row at a time:
+// 128 int8 values, or 32 values as 32 fp16 high halves followed by their 32 low halves.  In LDS a row of a tile is those 128
+// bytes = 8 pieces of 16 (one lane's MFMA operand); piece p of row r sits at p ^ (r & 7), so that the 32 rows that a wave
+// reads at one p spread over all banks (rows are 128 bytes apart: without it all 32 would start in the same bank).
+constexpr int TILE_KB = 128;
+__device__ inline int tile_off(int row, int piece) { return row * TILE_KB + ((piece ^ (row & 7)) << 4); }
+// 32x32 MFMA result: lane holds column (lane & 31) and, in register r, row
+__device__ inline int acc_row(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
+
+}  // namespace az

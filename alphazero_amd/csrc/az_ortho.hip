@@ -1,0 +1,384 @@
+// az_ortho.hip -- orthogonalisation of matrices by Newton-Schulz products, and the weight update around it.
+//
+//   X = G / (||G||_F + eps);   `steps` times:  A = X X^T,  B = a I + b A + c A^2,  X <- B X      (s x l, s <= l: G or G^T)
+//
+// Products are fp32-accurate on the fp16 matrix pipe: every operand is kept as hi + lo, two fp16 halves of the value times a
+// fixed power of two (X 2^14, A 2^12, B 2^11), and a product is hi hi + hi lo + lo hi with fp32 accumulation; the dropped
+// lo lo is 2^-22 of a product.  Singular values stay below 2 (the host checks the coefficients), so |X| <= 2, |A| <= 4 and
+// |B| <= 16 and no high half leaves fp16's range.  The fp32 pipe would be exact to 2^-24 and run at a sixteenth of the rate, 3
+// products at a third; one fp16 product (2^-11) is not enough: the iteration multiplies the rounding of X's small singular
+// directions by a^steps = 485.
+//
+// X is kept in both orientations, X [sp][lp] and T = X^T [lp][sp] (sp, lp: padded with zeros), because all three products
+// then read both operands along their rows:  A = X X^T,  A^2 = A A^T,  T <- T B  (A and B are symmetric).
+#include <math.h>
+
+#include "az_ops.hpp"
+
+namespace az {
+
+constexpr int OT = 64;             // tile edge and padding of s and l
+constexpr int MAX_JOBS = 16;       // matrices per set of launches (their table travels as a kernel argument)
+constexpr int MAX_PARTS = 512;     // partial sums of a norm
+constexpr i64 ORTHO_MAX_DIM = 32768;
+
+struct Job {
+    const void* g;   // gradient / input, [rows][cols]
+    float* m;        // momentum or null
+    void* w;         // weights (update) or output
+    i32 rows, cols, s, l, sp, lp, n_part;
+    float kappa;
+    double* part;
+    u8 *x, *t[2], *a, *b;   // split operands; a row of k values is k / 32 blocks of 128 bytes (32 hi, 32 lo)
+};
+struct Jobs {
+    Job j[MAX_JOBS];
+    i32 first[MAX_JOBS + 1];   // first block of every job in this launch
+    i32 n;
+};
+struct Hyper {
+    float mu, one_mu, decay, lr, a, b, c;
+    double eps;
+    int nesterov, update;   // update: the weight update; else out <- O(g)
+};
+
+__device__ inline int find_job(const Jobs& js, int block) {
+    int j = 0;
+    while (j + 1 < js.n && block >= js.first[j + 1]) j++;
+    return j;
+}
+template <class T>
+__device__ inline float update_value(const Job& J, const Hyper& h, i64 i) {   // after k_ortho_norm has updated m
+    const float g = to_f32(((const T*)J.g)[i]);
+    if (!h.update) return g;
+    const float m = J.m[i];
+    return h.nesterov ? h.mu * m + h.one_mu * g : m;
+}
+__device__ inline void split_store(u8* p, float v) {   // p: the high half's place
+    const f16 hi = (f16)v;
+    *(f16*)p = hi;
+    *(f16*)(p + 64) = (f16)(v - (float)hi);
+}
+__device__ inline float split_load(const u8* p) { return (float)*(const f16*)p + (float)*(const f16*)(p + 64); }
+__device__ inline i64 split_off(i64 row, i64 kp, i64 k) { return row * kp * 4 + (k >> 5) * TILE_KB + (k & 31) * 2; }
+
+// momentum (in place) and partial sums of squares of the update, in float64: the squares of float32 values can leave float32
+template <class T>
+__global__ __launch_bounds__(256) void k_ortho_norm(Jobs js, Hyper h) {
+    __shared__ double red[4];
+    const int ji = find_job(js, blockIdx.x);
+    const Job& J = js.j[ji];
+    const int part = blockIdx.x - js.first[ji];
+    const i64 n = (i64)J.rows * J.cols, per = (n + J.n_part - 1) / J.n_part, lo = part * per;
+    const i64 hi = lo + per < n ? lo + per : n;
+    double sum = 0;
+    for (i64 i = lo + threadIdx.x; i < hi; i += 256) {
+        if (h.update) J.m[i] = h.mu * J.m[i] + h.one_mu * to_f32(((const T*)J.g)[i]);
+        const double u = update_value<T>(J, h, i);
+        sum += u * u;
+    }
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) J.part[part] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// X and T from the update, padding included: one 64 x 64 tile per workgroup
+template <class T>
+__global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
+    __shared__ float tile[OT][OT + 1];   // [short index][long index]
+    __shared__ double red[4];
+    const int ji = find_job(js, blockIdx.x), tid = threadIdx.x;
+    const Job& J = js.j[ji];
+    const int nl = J.lp / OT, tl = blockIdx.x - js.first[ji], i0 = tl / nl * OT, j0 = tl % nl * OT;
+    double sum = 0;
+    for (int i = tid; i < J.n_part; i += 256) sum += J.part[i];
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if ((tid & 63) == 0) red[tid >> 6] = sum;
+    __syncthreads();
+    const float scale = (float)(16384.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + h.eps));
+    const bool flip = J.rows > J.cols;
+    for (int e = tid; e < OT * OT; e += 256) {
+        const int hi_ = e / OT, lo_ = e % OT;           // lo_ runs along the matrix's rows in memory
+        const int i = flip ? lo_ : hi_, j = flip ? hi_ : lo_;
+        float v = 0;
+        if (i0 + i < J.s && j0 + j < J.l)
+            v = update_value<T>(J, h, flip ? (i64)(j0 + j) * J.cols + i0 + i : (i64)(i0 + i) * J.cols + j0 + j) * scale;
+        tile[i][j] = v;
+    }
+    __syncthreads();
+    for (int e = tid; e < OT * OT; e += 256) {
+        const int r = e / OT, c = e % OT;
+        split_store(J.x + split_off(i0 + r, J.lp, j0 + c), tile[r][c]);
+        split_store(J.t[0] + split_off(j0 + r, J.sp, i0 + c), tile[c][r]);
+    }
+}
+
+// D[m][n] = sum_k P[m][k] Q[n][k] over split operands, 64 x 64 per workgroup, 4 waves of 32 x 32
+__device__ inline void split_product(const u8* P, const u8* Q, i64 m0, i64 n0, int kp, u8* tp, u8* tq, f32x16& acc) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
+    const i64 pitch = (i64)kp * 4;
+    for (int k0 = 0; k0 < kp; k0 += 32) {
+        for (int i = 0; i < 2; i++) {
+            const int row = (tid >> 3) + 32 * i, piece = tid & 7;
+            *(u32x4*)(tp + tile_off(row, piece)) = *(const u32x4*)(P + (m0 + row) * pitch + (i64)k0 * 4 + piece * 16);
+            *(u32x4*)(tq + tile_off(row, piece)) = *(const u32x4*)(Q + (n0 + row) * pitch + (i64)k0 * 4 + piece * 16);
+        }
+        __syncthreads();
+        for (int ks = 0; ks < 2; ks++) {
+            const int piece = 2 * ks + (lane >> 5), ra = wm + (lane & 31), rb = wn + (lane & 31);
+            const f16x8 ah = *(const f16x8*)(tp + tile_off(ra, piece)), al = *(const f16x8*)(tp + tile_off(ra, piece + 4));
+            const f16x8 bh = *(const f16x8*)(tq + tile_off(rb, piece)), bl = *(const f16x8*)(tq + tile_off(rb, piece + 4));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+        }
+        __syncthreads();
+    }
+}
+
+enum { GRAM = 0, POLY = 1, STEP = 2, LAST = 3 };
+
+template <int MODE, class T>
+__global__ __launch_bounds__(256) void k_ortho_product(Jobs js, Hyper h, int cur) {
+    __shared__ __attribute__((aligned(16))) u8 tp[OT * TILE_KB], tq[OT * TILE_KB];
+    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const Job& J = js.j[ji];
+    const int tl = blockIdx.x - js.first[ji];
+    const bool flip = J.rows > J.cols;
+    const u8 *P, *Q;
+    int kp, nt;
+    if (MODE == GRAM) { P = Q = J.x; kp = J.lp; nt = J.sp / OT; }
+    else if (MODE == POLY) { P = Q = J.a; kp = J.sp; nt = J.sp / OT; }
+    else if (MODE == STEP || flip) { P = J.t[cur]; Q = J.b; kp = J.sp; nt = J.sp / OT; }
+    else { P = J.b; Q = J.t[cur]; kp = J.sp; nt = J.lp / OT; }   // the output's own orientation
+    const i64 m0 = (i64)(tl / nt) * OT, n0 = (i64)(tl % nt) * OT;
+    f32x16 acc = {};
+    split_product(P, Q, m0, n0, kp, tp, tq, acc);
+    const i64 n = n0 + (wave & 1) * 32 + (lane & 31);
+    for (int r = 0; r < 16; r++) {
+        const i64 m = m0 + (wave >> 1) * 32 + acc_row(r, lane);
+        if (MODE == GRAM) {
+            split_store(J.a + split_off(m, J.sp, n), acc[r] * 0x1p-16f);
+        } else if (MODE == POLY) {
+            const float A = split_load(J.a + split_off(m, J.sp, n)) * 0x1p-12f;
+            const float B = h.c * (acc[r] * 0x1p-24f) + h.b * A + (m == n ? h.a : 0.0f);
+            split_store(J.b + split_off(m, J.sp, n), B * 0x1p11f);
+        } else if (MODE == STEP) {
+            const float v = acc[r] * 0x1p-11f;
+            split_store(J.t[cur ^ 1] + split_off(m, J.sp, n), v);
+            split_store(J.x + split_off(n, J.lp, m), v);
+        } else if (m < J.rows && n < J.cols) {
+            float v = acc[r] * 0x1p-25f;
+            T* w = (T*)J.w + m * J.cols + n;
+            if (h.update) v = to_f32(*w) * h.decay - v * (h.lr * J.kappa);
+            *w = from_f32<T>(v);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------- host side
+static i64 pad(i64 n) { return (n + OT - 1) / OT * OT; }
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static bool dims_ok(i64 rows, i64 cols) { return rows >= 1 && cols >= 1 && rows <= ORTHO_MAX_DIM && cols <= ORTHO_MAX_DIM; }
+
+// lays a job's workspace out from `p` on (null: only counts) and returns its bytes
+static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
+    J.rows = (i32)rows;
+    J.cols = (i32)cols;
+    J.s = (i32)(rows < cols ? rows : cols);
+    J.l = (i32)(rows < cols ? cols : rows);
+    J.sp = (i32)pad(J.s);
+    J.lp = (i32)pad(J.l);
+    const i64 parts = (rows * cols + 4095) / 4096;
+    J.n_part = (i32)(parts < MAX_PARTS ? parts : MAX_PARTS);
+    J.kappa = (float)sqrt(rows > cols ? (double)rows / (double)cols : 1.0);
+    size_t off = 0;
+    auto take = [&](size_t n) {
+        char* r = p ? p + off : nullptr;
+        off += up256(n);
+        return (u8*)r;
+    };
+    J.part = (double*)take(J.n_part * sizeof(double));
+    J.x = take((size_t)J.sp * J.lp * 4);
+    J.t[0] = take((size_t)J.sp * J.lp * 4);
+    J.t[1] = take((size_t)J.sp * J.lp * 4);
+    J.a = take((size_t)J.sp * J.sp * 4);
+    J.b = take((size_t)J.sp * J.sp * 4);
+    return off;
+}
+
+// Which coefficients keep the halves in range: follows the largest singular value through the steps on a fine grid.
+static bool coeffs_ok(int steps, const double* k) {
+    if (!k || !isfinite(k[0]) || !isfinite(k[1]) || !isfinite(k[2])) return false;
+    double top = 1.0;
+    for (int it = 0; it < steps; it++) {
+        double next = 0;
+        for (int i = 0; i <= 4096; i++) {
+            const double x = top * i / 4096, x2 = x * x, poly = k[0] + k[1] * x2 + k[2] * x2 * x2;
+            if (fabs(poly) > 15.9 || fabs(poly - k[0]) > 15.9) return false;
+            next = fmax(next, fabs(poly * x));
+        }
+        top = next * 1.001;
+        if (top > 1.99) return false;
+    }
+    return true;
+}
+
+template <class F>
+static void each_first(Jobs& js, F blocks) {
+    js.first[0] = 0;
+    for (int i = 0; i < js.n; i++) js.first[i + 1] = js.first[i] + (i32)blocks(js.j[i]);
+}
+
+static int run_jobs(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
+    each_first(js, [](const Job& J) { return J.n_part; });
+    AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
+    each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
+    AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
+    int cur = 0;
+    for (int it = 0; it < steps; it++) {
+        each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.sp / OT); });
+        k_ortho_product<GRAM, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
+        k_ortho_product<POLY, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
+        each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
+        if (it + 1 < steps) {
+            k_ortho_product<STEP, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
+        } else {
+            AZ_DISPATCH_DTYPE(dtype, k_ortho_product<LAST, T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur));
+        }
+        cur ^= 1;
+    }
+    return launch_status("az_orthogonalize");
+}
+
+}  // namespace az
+
+using namespace az;
+
+extern "C" {
+
+size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols) {
+    if (batch < 1 || !dims_ok(rows, cols)) return 0;
+    Job J;
+    return plan(J, rows, cols, nullptr) * (size_t)(batch < MAX_JOBS ? batch : MAX_JOBS);
+}
+
+static int ortho_check(int dtype, int steps, const double* coeffs, double eps, const void* ws, size_t ws_bytes, size_t need) {
+    if (!dtype_ok(dtype)) return refuse("az_orthogonalize: unknown dtype");
+    if (steps < 1 || steps > 16) return refuse("az_orthogonalize: steps is 1..16");
+    if (!(eps > 0) || !isfinite(eps)) return refuse("az_orthogonalize: eps must be positive and finite");
+    if (!coeffs_ok(steps, coeffs)) return refuse("az_orthogonalize: these coefficients leave the range of the products");
+    if (ws_bytes < need || (need && (!ws || ((uintptr_t)ws & 255))))
+        return refuse("az_orthogonalize: workspace too small or not aligned to 256 bytes");
+    return AZ_OK;
+}
+
+int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int64_t cols, const void* g_dev, void* out_dev,
+                         int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes, void* stream) {
+    if (batch < 0 || !dims_ok(rows, cols)) return refuse("az_orthogonalize: bad shape (rows and cols are 1..32768)");
+    int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_orthogonalize_ws(batch, rows, cols));
+    if (rc != AZ_OK) return rc;
+    if (batch > 0 && (!g_dev || !out_dev)) return refuse("az_orthogonalize: null pointer");
+    DeviceScope dev(device);
+    if (dev.rc != AZ_OK || batch == 0) return dev.rc;
+    Hyper h = {};
+    h.a = (float)coeffs[0];
+    h.b = (float)coeffs[1];
+    h.c = (float)coeffs[2];
+    h.eps = eps;
+    const size_t bytes = (size_t)rows * cols * dtype_size(dtype);
+    for (int64_t lo = 0; lo < batch; lo += MAX_JOBS) {
+        Jobs js;
+        js.n = (i32)(batch - lo < MAX_JOBS ? batch - lo : MAX_JOBS);
+        size_t off = 0;
+        for (int i = 0; i < js.n; i++) {
+            Job& J = js.j[i];
+            off += plan(J, rows, cols, (char*)ws_dev + off);
+            J.g = (const char*)g_dev + (lo + i) * bytes;
+            J.w = (char*)out_dev + (lo + i) * bytes;
+            J.m = nullptr;
+        }
+        rc = run_jobs(js, h, steps, dtype, (hipStream_t)stream);
+        if (rc != AZ_OK) return rc;
+    }
+    return AZ_OK;
+}
+
+size_t az_muon_step_ws(const az_muon_item* items, int64_t n) {
+    size_t most = 0;
+    if (!items) return 0;
+    for (int64_t lo = 0; lo < n; lo += MAX_JOBS) {
+        size_t sum = 0;
+        for (int64_t i = lo; i < n && i < lo + MAX_JOBS; i++) {
+            Job J;
+            if (!dims_ok(items[i].rows, items[i].cols)) return 0;
+            sum += plan(J, items[i].rows, items[i].cols, nullptr);
+        }
+        most = sum > most ? sum : most;
+    }
+    return most;
+}
+
+int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n, double lr, double momentum, int nesterov,
+                     double weight_decay, int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes,
+                     void* stream) {
+    if (n < 0 || n > 65536 || (n > 0 && !items)) return refuse("az_muon_step: bad item list");
+    if (!dtype_ok(dtype)) return refuse("az_muon_step: unknown dtype");
+    for (int64_t i = 0; i < n; i++) {
+        if (!dims_ok(items[i].rows, items[i].cols)) return refuse("az_muon_step: bad shape (rows and cols are 1..32768)");
+        if (!items[i].w_dev || !items[i].g_dev || !items[i].m_dev) return refuse("az_muon_step: null pointer");
+    }
+    // what is written (w, m) overlaps nothing else
+    auto overlap = [](const void* p, size_t np, const void* q, size_t nq) {
+        return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+    };
+    for (int64_t i = 0; i < n; i++) {
+        const size_t ni = (size_t)items[i].rows * items[i].cols, es = dtype_size(dtype);
+        for (int64_t k = 0; k < n; k++) {
+            const size_t nk = (size_t)items[k].rows * items[k].cols;
+            if ((k < i && (overlap(items[i].w_dev, ni * es, items[k].w_dev, nk * es) ||
+                           overlap(items[i].m_dev, ni * 4, items[k].m_dev, nk * 4))) ||
+                overlap(items[i].w_dev, ni * es, items[k].m_dev, nk * 4) ||
+                overlap(items[i].g_dev, ni * es, items[k].w_dev, nk * es) ||
+                overlap(items[i].g_dev, ni * es, items[k].m_dev, nk * 4))
+                return refuse("az_muon_step: weights and momenta must not overlap each other or a gradient");
+        }
+    }
+    if (!isfinite(lr) || !isfinite(weight_decay) || !(momentum >= 0 && momentum < 1))
+        return refuse("az_muon_step: bad lr, weight_decay or momentum (0 <= momentum < 1)");
+    int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_muon_step_ws(items, n));
+    if (rc != AZ_OK) return rc;
+    DeviceScope dev(device);
+    if (dev.rc != AZ_OK || n == 0) return dev.rc;
+    Hyper h = {};
+    h.mu = (float)momentum;
+    h.one_mu = (float)(1.0 - momentum);
+    h.decay = (float)(1.0 - lr * weight_decay);
+    h.lr = (float)lr;
+    h.a = (float)coeffs[0];
+    h.b = (float)coeffs[1];
+    h.c = (float)coeffs[2];
+    h.eps = eps;
+    h.nesterov = nesterov != 0;
+    h.update = 1;
+    for (int64_t lo = 0; lo < n; lo += MAX_JOBS) {
+        Jobs js;
+        js.n = (i32)(n - lo < MAX_JOBS ? n - lo : MAX_JOBS);
+        size_t off = 0;
+        for (int i = 0; i < js.n; i++) {
+            const az_muon_item& it = items[lo + i];
+            Job& J = js.j[i];
+            off += plan(J, it.rows, it.cols, (char*)ws_dev + off);
+            J.g = it.g_dev;
+            J.w = it.w_dev;
+            J.m = it.m_dev;
+        }
+        rc = run_jobs(js, h, steps, dtype, (hipStream_t)stream);
+        if (rc != AZ_OK) return rc;
+    }
+    return AZ_OK;
+}
+
+}  // extern "C"

@@ -288,6 +288,69 @@ int az_net_get_kernel(az_engine *e);
 /* device-resident forward for bench.py / rocprof: states_dev [n][2], outputs device pointers, async. */
 int az_net_forward_dev(az_engine *e, int64_t n, const uint64_t *states_dev, float *probs_dev, float *value_dev);
 
+/* ---- operators on device tensors ------------------------------------------------------------------------- */
+/* For networks and training steps of the caller's own around the engine (a network that K3 does not know is evaluated
+ * between az_select and az_backup; its weights are trained outside).  Pointers ending in _dev are memory of `device`;
+ * every call is asynchronous on `stream` (a hipStream_t of that device; NULL = its default stream), allocates nothing,
+ * keeps nothing and may be captured into a HIP graph.  Calls may overlap in time if their outputs and workspaces do not.
+ * `ws_dev`: workspace of at least the bytes that the matching *_ws function returns, aligned to 256 bytes, contents
+ * irrelevant before and after; less than that is AZ_ERR_ARG.  The caller's current device is restored. */
+#define AZ_F32 0
+#define AZ_F16 1
+#define AZ_BF16 2
+#define AZ_ACT_NONE 0
+#define AZ_ACT_RELU 1
+#define AZ_ACT_SILU 2
+
+/* Rows as 8-bit integers with one scale each:  scale = max|x| * (1/127) in float32,  q = x / scale rounded to the nearest
+ * integer (ties to even, by the exact quotient), |q| <= 127.  A row of zeros has scale 0 and q = 0; a row that holds a
+ * NaN or an infinity has scale NaN and q = 0, so that what is computed from it is NaN.
+ * index_dev == NULL: row r of q is row r of x (n_src rows of `cols` elements, ld_x elements apart).  Else index_dev is
+ * [rows][taps] and row r of q is the `taps` rows x[index[r][0]], x[index[r][1]], ... one after the other, taps * cols
+ * values under one scale (the rows of a convolution); an index outside [0, n_src) stands for a row of zeros.
+ * ld_q: bytes from row to row of q, at least taps * cols; the bytes between are not written.  taps * cols < 2^31. */
+int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const void *x_dev, int64_t ld_x, int64_t n_src,
+                       const int32_t *index_dev, int32_t taps, int8_t *q_dev, int64_t ld_q, float *scale_dev,
+                       void *stream);
+/* y[m][n] = act(q_scale[m] * w_scale[n] * sum_k q[m][k] w[n][k] + bias[n] + residual[m][n]), integer sums exact, the rest
+ * in float32, rounded once to `dtype` (of y and residual).  bias and residual may be NULL; residual may be y itself.
+ * ld_*: elements from row to row.  k <= 131071 (above that a sum could leave int32). */
+size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k);
+int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t *q_dev, int64_t ld_q,
+                     const float *q_scale_dev, const int8_t *w_dev, int64_t ld_w, const float *w_scale_dev,
+                     const float *bias_dev, const void *residual_dev, int64_t ld_res, int act, int dtype, void *y_dev,
+                     int64_t ld_y, void *ws_dev, size_t ws_bytes, void *stream);
+/* az_i8_quantize_dev followed by az_i8_matmul_dev on rows x[m][k] of `dtype`, ld_x elements apart. */
+size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k);
+int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void *x_dev, int64_t ld_x, const int8_t *w_dev,
+                     int64_t ld_w, const float *w_scale_dev, const float *bias_dev, const void *residual_dev,
+                     int64_t ld_res, int act, int dtype, void *y_dev, int64_t ld_y, void *ws_dev, size_t ws_bytes,
+                     void *stream);
+
+/* Orthogonalisation of `batch` matrices [rows][cols] (contiguous) by Newton-Schulz products: X = G / (||G||_F + eps), then
+ * `steps` times X <- a X + (b A + c A^2) X with A = X X^T (on the shorter side), coeffs = {a, b, c}.  Products are
+ * float32-accurate (fp16 matrix pipe, operands split into two halves); out may be g.  steps 1..16, eps > 0.  Coefficients whose
+ * iteration takes a singular value of [0, 1] above 2, or b A + c A^2 + a out of [-16, 16], are AZ_ERR_ARG (the halves' range).
+ * A matrix that holds a NaN or an infinity comes out as NaN.  rows, cols <= 32768. */
+size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols);
+int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *g_dev, void *out_dev,
+                         int steps, const double *coeffs, double eps, void *ws_dev, size_t ws_bytes, void *stream);
+/* One update of n weight matrices by orthogonalised momentum, for each item:
+ *   m <- momentum m + (1 - momentum) g;   u = nesterov ? momentum m + (1 - momentum) g : m
+ *   w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) O(u),   O = the orthogonalisation above
+ * w and g of `dtype`, m float32, each contiguous [rows][cols].  items is a host array (n <= 65536), read before the
+ * call returns; no w or m may overlap another item's or a gradient. */
+typedef struct az_muon_item {
+    void *w_dev;
+    const void *g_dev;
+    float *m_dev;
+    int64_t rows, cols;
+} az_muon_item;
+size_t az_muon_step_ws(const az_muon_item *items, int64_t n);
+int az_muon_step_dev(int device, int dtype, const az_muon_item *items, int64_t n, double lr, double momentum, int nesterov,
+                     double weight_decay, int steps, const double *coeffs, double eps, void *ws_dev, size_t ws_bytes,
+                     void *stream);
+
 /* ---- test hooks ------------------------------------------------------------------------------------------ */
 /* replace every slot's tree by a root whose children, in this insertion order, have these actions and visit counts
  * (arrays [G][A], n_children[G]), so that az_choose_moves can be checked against recorded outputs of
