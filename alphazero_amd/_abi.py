@@ -100,10 +100,10 @@ SIGNATURES = {
     "az_net_get_kernel": (C.c_int, [_vp]),
     "az_net_forward_dev": (C.c_int, [_vp, _i64, _vp, _vp, _vp]),
     "az_i8_quantize_dev": (C.c_int, [C.c_int, C.c_int, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp, _i64, _vp, _vp]),
-    "az_i8_matmul_ws": (C.c_size_t, [_i64, _i64, _i64]),
+    "az_i8_matmul_ws": (C.c_size_t, [_i64, _i64, _i64, _vp, _i64, _vp, _i64]),
     "az_i8_matmul_dev": (C.c_int, [C.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp, _i64, C.c_int,
                                    C.c_int, _vp, _i64, _vp, C.c_size_t, _vp]),
-    "az_i8_linear_ws": (C.c_size_t, [_i64, _i64, _i64]),
+    "az_i8_linear_ws": (C.c_size_t, [_i64, _i64, _i64, _vp, _i64]),
     "az_i8_linear_dev": (C.c_int, [C.c_int, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, C.c_int, C.c_int,
                                    _vp, _i64, _vp, C.c_size_t, _vp]),
     "az_orthogonalize_ws": (C.c_size_t, [_i64, _i64, _i64]),

@@ -6,7 +6,7 @@
 // The sums are int32 and exact (|q w| <= 2^14, k <= 131071), so no order of summation changes a result.
 #include <math.h>
 
-#include "az_ops.hpp"
+#include "az_tile.hpp"
 
 namespace az {
 
@@ -88,6 +88,7 @@ struct Mm {
     void* y;
     i64 ld_y;
     int act;
+    bool pair_store;   // every even column of y starts at a multiple of two elements
 };
 
 __device__ inline float activate(float v, int act) {
@@ -109,50 +110,244 @@ __device__ inline u32x4 load_piece(const i8* row, i64 k, i64 K) {
     return v;
 }
 
-// 64 x 64 outputs per workgroup, 4 waves of 32 x 32, any alignment
 template <class T>
-__global__ __launch_bounds__(256) void k_i8_mm_any(Mm p) {
-    __shared__ __attribute__((aligned(16))) u8 ta[64 * TILE_KB], tb[64 * TILE_KB];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const i64 tiles_n = (p.n + 63) / 64;
-    const i64 m0 = (i64)blockIdx.x / tiles_n * 64, n0 = (i64)blockIdx.x % tiles_n * 64;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    i32x16 acc = {};
-    for (i64 k0 = 0; k0 < p.k; k0 += TILE_KB) {
-        for (int i = 0; i < 2; i++) {
-            const int row = (tid >> 3) + 32 * i, piece = tid & 7;
-            const u32x4 zero = {0, 0, 0, 0};
-            const u32x4 a = m0 + row < p.m ? load_piece(p.q + (m0 + row) * p.ld_q, k0 + piece * 16, p.k) : zero;
-            const u32x4 b = n0 + row < p.n ? load_piece(p.w + (n0 + row) * p.ld_w, k0 + piece * 16, p.k) : zero;
-            *(u32x4*)(ta + tile_off(row, piece)) = a;
-            *(u32x4*)(tb + tile_off(row, piece)) = b;
-        }
-        __syncthreads();
-        for (int ks = 0; ks < 4; ks++) {
-            const int piece = 2 * ks + (lane >> 5);
-            const i32x4 a = *(const i32x4*)(ta + tile_off(wm + (lane & 31), piece));
-            const i32x4 b = *(const i32x4*)(tb + tile_off(wn + (lane & 31), piece));
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(a, b, acc, 0, 0, 0);
-        }
-        __syncthreads();
+__device__ inline void put(const Mm& p, i64 m, i64 n, int sum) {
+    float v = (float)sum * p.qs[m] * p.ws[n] + (p.bias ? p.bias[n] : 0.0f);
+    if (p.res) v += to_f32(((const T*)p.res)[m * p.ld_res + n]);
+    ((T*)p.y)[m * p.ld_y + n] = from_f32<T>(activate(v, p.act));
+}
+
+// Rows of both operands at multiples of 16 bytes, k a multiple of 16.  blockIdx.y: which of the `splits` parts of k (whole
+// steps each); with more than one the int32 sums go to part[split][m][n] and k_i8_join adds them.
+template <class T, class S>
+__global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u32 tiles_n, u32 steps_per_split, int* part) {
+    extern __shared__ __attribute__((aligned(128))) u8 lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    u32 tm, tn;
+    tile_place(blockIdx.x, tiles_m, tiles_n, tm, tn);
+    const i64 m0 = (i64)tm * S::BM, n0 = (i64)tn * S::BN;
+    auto span = [](i64 rows, i64 most, i64 ld, i64 k) {   // bytes from the first row on that belong to the operand
+        const i64 r = rows < most ? rows : most;
+        return (u32)((r - 1) * ld + k);
+    };
+    const TileSrc<false> a(p.q + m0 * p.ld_q, (u32)p.ld_q, span(p.m - m0, S::BM, p.ld_q, p.k), lane);
+    const TileSrc<S::PAIRS> b(p.w + n0 * p.ld_w, (u32)p.ld_w, span(p.n - n0, S::BN, p.ld_w, p.k), lane);
+    const u32 k0 = blockIdx.y * steps_per_split * TILE_KB;
+    u32 kend = k0 + steps_per_split * TILE_KB;
+    kend = kend < (u32)p.k ? kend : (u32)p.k;
+    i32x16 acc[S::FM][S::FN] = {};
+    tile_product<KindI8, S>(KindI8(), a, b, k0, kend, lds, wave, lane, acc);
+    // scales of the tile's rows and columns through LDS (its tiles have been read)
+    float *sm = (float*)lds, *sn = sm + S::BM, *bn = sn + S::BN;
+    for (int t = threadIdx.x; t < S::BM; t += S::THREADS) sm[t] = p.qs[m0 + t < p.m ? m0 + t : p.m - 1];
+    for (int t = threadIdx.x; t < S::BN; t += S::THREADS) {
+        const i64 n = n0 + t < p.n ? n0 + t : p.n - 1;
+        sn[t] = p.ws[n];
+        bn[t] = p.bias ? p.bias[n] : 0.0f;
     }
-    const i64 n = n0 + wn + (lane & 31);
+    __syncthreads();
+    const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32), c = S::PAIRS ? 2 * (lane & 31) : lane & 31;
+    const i64 n = n0 + wn + c;
+    const float s0 = sn[wn + c], b0 = bn[wn + c], s1 = S::PAIRS ? sn[wn + c + 1] : 0, b1 = S::PAIRS ? bn[wn + c + 1] : 0;
     if (n >= p.n) return;
-    const float sw = p.ws[n], bias = p.bias ? p.bias[n] : 0.0f;
-    for (int r = 0; r < 16; r++) {
-        const i64 m = m0 + wm + acc_row(r, lane);
-        if (m >= p.m) continue;
-        float v = (float)acc[r] * p.qs[m] * sw + bias;
-        if (p.res) v += to_f32(((const T*)p.res)[m * p.ld_res + n]);
-        ((T*)p.y)[m * p.ld_y + n] = from_f32<T>(activate(v, p.act));
+    const bool two = S::PAIRS && n + 1 < p.n;
+    if (part) part += (i64)blockIdx.y * p.m * p.n;
+#pragma unroll
+    for (int i = 0; i < S::FM; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const int row = wm + 32 * i + acc_row(4 * g, lane);
+            const f32x4 s4 = *(const f32x4*)(sm + row);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const i64 m = m0 + row + e;
+                if (m >= p.m) break;
+                const int q0 = acc[i][0][4 * g + e], q1 = acc[i][S::FN - 1][4 * g + e];
+                if (part) {
+                    part[m * p.n + n] = q0;
+                    if (two) part[m * p.n + n + 1] = q1;
+                    continue;
+                }
+                float v0 = (float)q0 * s4[e] * s0 + b0, v1 = (float)q1 * s4[e] * s1 + b1;
+                T* y = (T*)p.y + m * p.ld_y + n;
+                if (p.res) {
+                    const T* r = (const T*)p.res + m * p.ld_res + n;
+                    v0 += to_f32(r[0]);
+                    if (two) v1 += to_f32(r[1]);
+                }
+                v0 = activate(v0, p.act);
+                if (S::PAIRS && two && p.pair_store) {
+                    struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
+                    *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate(v1, p.act))};
+                } else {
+                    y[0] = from_f32<T>(v0);
+                    if (two) y[1] = from_f32<T>(activate(v1, p.act));
+                }
+            }
+        }
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __restrict__ part) {
+    const i64 total = p.m * p.n;
+    for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
+        int sum = 0;
+        for (u32 s = 0; s < splits; s++) sum += part[s * total + e];
+        put<T>(p, e / p.n, e % p.n, sum);
     }
 }
 
-static int i8_matmul(const Mm& p, int dtype, void* ws, size_t ws_bytes, hipStream_t st) {
-    const i64 tiles = ((p.m + 63) / 64) * ((p.n + 63) / 64);
-    if (tiles > 0x7fffffff) return refuse("az_i8_matmul: more than 2^31 tiles");
-    AZ_DISPATCH_DTYPE(dtype, k_i8_mm_any<T><<<dim3((u32)tiles), dim3(256), 0, st>>>(p));
+// Few rows (m <= 16 FM): a workgroup's 8 waves share 16 channels and split k between them, 64 bytes of a row a step, and add
+// their int32 sums in LDS.  What bounds it is reading w once: each wave asks for its share of 16 rows, 64 contiguous bytes of
+// a row per 4 lanes, with nothing between the loads.  Any alignment.
+constexpr int FEW_WAVES = 8;
+template <class T, int FM>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_mm_few(Mm p) {
+    __shared__ int sums[FEW_WAVES][FM * 16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, quarter = lane >> 4;
+    const i64 n0 = (i64)blockIdx.x * 16, n = n0 + row < p.n ? n0 + row : p.n - 1;   // rows behind the last: the last again
+    const i8* w = p.w + n * p.ld_w;
+    const i8* q[FM];
+#pragma unroll
+    for (int f = 0; f < FM; f++) q[f] = p.q + (16 * f + row < p.m ? 16 * f + row : p.m - 1) * p.ld_q;
+    i32x4 acc[FM] = {};
+    const i64 whole = p.k & ~(i64)63;
+#pragma unroll 4
+    for (i64 k = wave * 64; k < whole; k += FEW_WAVES * 64) {
+        i32x4 b, a[FM];
+        __builtin_memcpy(&b, w + k + quarter * 16, 16);
+#pragma unroll
+        for (int f = 0; f < FM; f++) __builtin_memcpy(&a[f], q[f] + k + quarter * 16, 16);
+#pragma unroll
+        for (int f = 0; f < FM; f++) acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[f], b, acc[f], 0, 0, 0);
+    }
+    if (whole < p.k && wave == (int)(whole / 64 % FEW_WAVES)) {
+        const i32x4 b = __builtin_bit_cast(i32x4, load_piece(w, whole + quarter * 16, p.k));
+#pragma unroll
+        for (int f = 0; f < FM; f++) {
+            const i32x4 a = __builtin_bit_cast(i32x4, load_piece(q[f], whole + quarter * 16, p.k));
+            acc[f] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc[f], 0, 0, 0);
+        }
+    }
+    // 16x16 result: lane holds column (channel) lane & 15 and rows 4 (lane >> 4) + r
+#pragma unroll
+    for (int f = 0; f < FM; f++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) sums[wave][16 * f + 4 * quarter + r][row] = acc[f][r];
+    __syncthreads();
+    for (int e = threadIdx.x; e < FM * 256; e += 64 * FEW_WAVES) {
+        const int m = e >> 4, c = e & 15;
+        if (m >= p.m || n0 + c >= p.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < FEW_WAVES; i++) sum += sums[i][m][c];
+        put<T>(p, m, n0 + c, sum);
+    }
+}
+
+// Rows of k bytes at any address -> rows of kp (a multiple of 16) with zeros behind k.  16 output bytes a thread.
+__global__ __launch_bounds__(256) void k_i8_align(const i8* __restrict__ src, i64 ld, i64 rows, i64 k, i64 kp, i8* __restrict__ dst) {
+    const i64 pieces = kp / 16, total = rows * pieces;
+    for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
+        const i64 r = e / pieces, c = (e - r * pieces) * 16;
+        *(u32x4*)(dst + r * kp + c) = load_piece(src + r * ld, c, k);
+    }
+}
+
+static bool pairs_ok(const void* y, i64 ld_y, int dtype) { return ld_y % 2 == 0 && (uintptr_t)y % (2 * dtype_size(dtype)) == 0; }
+static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static i64 up(i64 n, i64 to) { return (n + to - 1) / to * to; }
+
+constexpr i64 FEW_ROWS = 64;          // up to this many rows of q: k_i8_mm_few
+constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
+
+using Tile256 = TileShape<256, 256, 2, 4, 4>;
+using Tile128 = TileShape<128, 128, 2, 2, 4>;
+using Tile64 = TileShape<64, 64, 2, 2, 4>;
+
+// How a product is computed; a function of the sizes and alignments alone, so that the workspace can be asked for first.
+struct MmPlan {
+    int tile;            // 0: few rows; 64, 128, 256: tile edge
+    bool align_q, align_w;
+    u32 splits, steps_per_split;
+    i64 kp;              // row length of aligned copies
+    size_t q_bytes, w_bytes, part_bytes;
+    size_t total() const { return q_bytes + w_bytes + part_bytes; }
+};
+static MmPlan mm_plan(i64 m, i64 n, i64 k, const void* q, i64 ld_q, const void* w, i64 ld_w) {
+    MmPlan P = {};
+    P.splits = 1;
+    P.kp = up(k, 16);
+    if (m <= FEW_ROWS) return P;
+    // the loads into LDS move 16 aligned bytes; rows whose length is no multiple of 16 need zeros behind them in one operand
+    P.align_q = ((uintptr_t)q & 15) || (ld_q & 15) || (k & 15) || ld_q > TILE_MAX_LD;
+    P.align_w = ((uintptr_t)w & 15) || (ld_w & 15) || ld_w > TILE_MAX_LD;
+    P.q_bytes = P.align_q ? up256((size_t)m * P.kp) : 0;
+    P.w_bytes = P.align_w ? up256((size_t)n * P.kp) : 0;
+    auto tiles = [&](i64 e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
+    // a larger tile reads less per product, but must not be mostly padding and must fill the chip
+    auto pays = [&](i64 e) { return tiles(e) >= 200 && tiles(e) * e * e <= tiles(e / 2) * (e / 2) * (e / 2) * 9 / 8; };
+    P.tile = pays(256) ? 256 : pays(128) ? 128 : 64;
+    const u32 steps = (u32)((k + TILE_KB - 1) / TILE_KB);
+    u32 splits = 1;
+    if (P.tile == 64)
+        while (splits < 16 && tiles(64) * splits * 2 <= 512 && steps / (splits * 2) >= 4) splits *= 2;
+    P.steps_per_split = (steps + splits - 1) / splits;
+    P.splits = (steps + P.steps_per_split - 1) / P.steps_per_split;
+    P.part_bytes = P.splits > 1 ? up256((size_t)P.splits * m * n * 4) : 0;
+    return P;
+}
+
+template <class T, class S>
+static int launch_tile(const Mm& p, const MmPlan& P, int* part, hipStream_t st) {
+    const i64 tm = (p.m + S::BM - 1) / S::BM, tn = (p.n + S::BN - 1) / S::BN;
+    if (tm * tn > 0x7fffffff) return refuse("az_i8_matmul: more than 2^31 tiles");
+    if (S::LDS > 64 * 1024) {
+        hipError_t e = hipFuncSetAttribute((const void*)k_i8_mm_tile<T, S>, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            set_error("az_i8_matmul: hipFuncSetAttribute failed");
+            return AZ_ERR_HIP;
+        }
+    }
+    k_i8_mm_tile<T, S><<<dim3((u32)(tm * tn), P.splits), dim3(S::THREADS), S::LDS, st>>>(p, (u32)tm, (u32)tn, P.steps_per_split, part);
+    if (part) {
+        const i64 blocks = (p.m * p.n + 255) / 256;
+        k_i8_join<T><<<dim3((u32)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st>>>(p, P.splits, part);
+    }
     return launch_status("az_i8_matmul");
+}
+
+template <class T>
+static int mm_launch(Mm p, const MmPlan& P, char* ws, hipStream_t st) {
+    if (P.tile == 0) {
+        const i64 blocks = (p.n + 15) / 16;
+        if (blocks > 0x7fffffff) return refuse("az_i8_matmul: more than 2^31 tiles");
+        const dim3 grid((u32)blocks), block(64 * FEW_WAVES);
+        if (p.m <= 16) k_i8_mm_few<T, 1><<<grid, block, 0, st>>>(p);
+        else if (p.m <= 32) k_i8_mm_few<T, 2><<<grid, block, 0, st>>>(p);
+        else if (p.m <= 48) k_i8_mm_few<T, 3><<<grid, block, 0, st>>>(p);
+        else k_i8_mm_few<T, 4><<<grid, block, 0, st>>>(p);
+        return launch_status("az_i8_matmul");
+    }
+    auto align = [&](const i8*& src, i64& ld, i64 rows, char* dst) {
+        const i64 blocks = (rows * (P.kp / 16) + 255) / 256;
+        k_i8_align<<<dim3((u32)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st>>>(src, ld, rows, p.k, P.kp, (i8*)dst);
+        src = (const i8*)dst;
+        ld = P.kp;
+    };
+    if (P.align_q) align(p.q, p.ld_q, p.m, ws);
+    if (P.align_w) align(p.w, p.ld_w, p.n, ws + P.q_bytes);
+    p.k = P.kp;   // from here on with the zeros (of one operand at least) behind the end
+    int* part = P.splits > 1 ? (int*)(ws + P.q_bytes + P.w_bytes) : nullptr;
+    if (P.tile == 256) return launch_tile<T, Tile256>(p, P, part, st);
+    if (P.tile == 128) return launch_tile<T, Tile128>(p, P, part, st);
+    return launch_tile<T, Tile64>(p, P, part, st);
+}
+
+static int i8_matmul(const Mm& p, int dtype, void* ws, hipStream_t st) {
+    const MmPlan P = mm_plan(p.m, p.n, p.k, p.q, p.ld_q, p.w, p.ld_w);
+    AZ_DISPATCH_DTYPE(dtype, return mm_launch<T>(p, P, (char*)ws, st));
+    return AZ_OK;
 }
 
 static int i8_quantize(int dtype, i64 rows, i64 cols, const void* x, i64 ld_x, i64 n_src, const i32* index, int taps, i8* q,
@@ -164,7 +359,6 @@ static int i8_quantize(int dtype, i64 rows, i64 cols, const void* x, i64 ld_x, i
 }
 
 static i64 linear_pitch(i64 k) { return (k + 15) & ~(i64)15; }
-static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 }  // namespace az
 
@@ -199,7 +393,10 @@ static int mm_check(int64_t m, int64_t n, int64_t k, int64_t ld_x, int64_t ld_w,
     return AZ_OK;
 }
 
-size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k) { return 0; }
+size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k, const int8_t* q_dev, int64_t ld_q, const int8_t* w_dev, int64_t ld_w) {
+    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K) return 0;
+    return mm_plan(m, n, k, q_dev, ld_q, w_dev, ld_w).total();
+}
 
 int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t* q_dev, int64_t ld_q,
                      const float* q_scale_dev, const int8_t* w_dev, int64_t ld_w, const float* w_scale_dev,
@@ -207,18 +404,21 @@ int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t* 
                      int64_t ld_y, void* ws_dev, size_t ws_bytes, void* stream) {
     const int rc = mm_check(m, n, k, ld_q, ld_w, residual_dev, ld_res, act, dtype, ld_y);
     if (rc != AZ_OK) return rc;
-    if (ws_bytes < az_i8_matmul_ws(m, n, k)) return refuse("az_i8_matmul: workspace too small");
+    const size_t need = az_i8_matmul_ws(m, n, k, q_dev, ld_q, w_dev, ld_w);
+    if (ws_bytes < need || (need && (!ws_dev || ((uintptr_t)ws_dev & 255))))
+        return refuse("az_i8_matmul: workspace too small or not aligned to 256 bytes");
     if (m > 0 && n > 0 && (!q_dev || !q_scale_dev || !w_dev || !w_scale_dev || !y_dev))
         return refuse("az_i8_matmul: null pointer");
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || m == 0 || n == 0) return dev.rc;
-    const Mm p = {m, n, k, q_dev, w_dev, ld_q, ld_w, q_scale_dev, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act};
-    return i8_matmul(p, dtype, ws_dev, ws_bytes, (hipStream_t)stream);
+    const Mm p = {m, n, k, q_dev, w_dev, ld_q, ld_w, q_scale_dev, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act, pairs_ok(y_dev, ld_y, dtype)};
+    return i8_matmul(p, dtype, ws_dev, (hipStream_t)stream);
 }
 
-size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k) {
+size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k, const int8_t* w_dev, int64_t ld_w) {
     if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K) return 0;
-    return up256((size_t)m * linear_pitch(k)) + up256((size_t)m * 4) + az_i8_matmul_ws(m, n, k);
+    return up256((size_t)m * linear_pitch(k)) + up256((size_t)m * 4) +
+           mm_plan(m, n, k, nullptr, linear_pitch(k), w_dev, ld_w).total();
 }
 
 int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void* x_dev, int64_t ld_x, const int8_t* w_dev,
@@ -227,7 +427,7 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void* x_
                      void* stream) {
     int rc = mm_check(m, n, k, ld_x, ld_w, residual_dev, ld_res, act, dtype, ld_y);
     if (rc != AZ_OK) return rc;
-    const size_t need = az_i8_linear_ws(m, n, k);
+    const size_t need = az_i8_linear_ws(m, n, k, w_dev, ld_w);
     if (ws_bytes < need || (need && (!ws_dev || ((uintptr_t)ws_dev & 255))))
         return refuse("az_i8_linear: workspace too small or not aligned to 256 bytes");
     if (m > 0 && n > 0 && (!x_dev || !w_dev || !w_scale_dev || !y_dev)) return refuse("az_i8_linear: null pointer");
@@ -239,8 +439,8 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void* x_
     char* rest = (char*)qs + up256((size_t)m * 4);
     rc = i8_quantize(dtype, m, k, x_dev, ld_x, m, nullptr, 1, q, linear_pitch(k), qs, st);
     if (rc != AZ_OK) return rc;
-    const Mm p = {m, n, k, q, w_dev, linear_pitch(k), ld_w, qs, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act};
-    return i8_matmul(p, dtype, rest, ws_bytes - (rest - (char*)ws_dev), st);
+    const Mm p = {m, n, k, q, w_dev, linear_pitch(k), ld_w, qs, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act, pairs_ok(y_dev, ld_y, dtype)};
+    return i8_matmul(p, dtype, rest, st);
 }
 
 }  // extern "C"

@@ -76,14 +76,4 @@ inline int refuse(const char* what) {
     return AZ_ERR_ARG;
 }
 
-// ---- matrix tiles ----------------------------------------------------------------------------------------------------
-// Both products (int8, and fp32 as split fp16) read their operands along the reduction axis, 128 bytes of a row at a time:
-// 128 int8 values, or 32 values as 32 fp16 high halves followed by their 32 low halves.  In LDS a row of a tile is those 128
-// bytes = 8 pieces of 16 (one lane's MFMA operand); piece p of row r sits at p ^ (r & 7), so that the 32 rows that a wave
-// reads at one p spread over all banks (rows are 128 bytes apart: without it all 32 would start in the same bank).
-constexpr int TILE_KB = 128;
-__device__ inline int tile_off(int row, int piece) { return row * TILE_KB + ((piece ^ (row & 7)) << 4); }
-// 32x32 MFMA result: lane holds column (lane & 31) and, in register r, row
-__device__ inline int acc_row(int r, int lane) { return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3); }
-
 }  // namespace az

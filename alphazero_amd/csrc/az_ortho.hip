@@ -13,11 +13,11 @@
 // then read both operands along their rows:  A = X X^T,  A^2 = A A^T,  T <- T B  (A and B are symmetric).
 #include <math.h>
 
-#include "az_ops.hpp"
+#include "az_tile.hpp"
 
 namespace az {
 
-constexpr int OT = 64;             // tile edge and padding of s and l
+constexpr int OT = 64;             // padding of s and l
 constexpr int MAX_JOBS = 16;       // matrices per set of launches (their table travels as a kernel argument)
 constexpr int MAX_PARTS = 512;     // partial sums of a norm
 constexpr i64 ORTHO_MAX_DIM = 32768;
@@ -29,7 +29,7 @@ struct Job {
     i32 rows, cols, s, l, sp, lp, n_part;
     float kappa;
     double* part;
-    u8 *x, *t[2], *a, *b;   // split operands; a row of k values is k / 32 blocks of 128 bytes (32 hi, 32 lo)
+    u8 *x, *t[2], *a, *b;   // split operands; a row of k values is k / 16 blocks of 64 bytes (16 hi, 16 lo)
 };
 struct Jobs {
     Job j[MAX_JOBS];
@@ -57,10 +57,10 @@ __device__ inline float update_value(const Job& J, const Hyper& h, i64 i) {   //
 __device__ inline void split_store(u8* p, float v) {   // p: the high half's place
     const f16 hi = (f16)v;
     *(f16*)p = hi;
-    *(f16*)(p + 64) = (f16)(v - (float)hi);
+    *(f16*)(p + 32) = (f16)(v - (float)hi);
 }
-__device__ inline float split_load(const u8* p) { return (float)*(const f16*)p + (float)*(const f16*)(p + 64); }
-__device__ inline i64 split_off(i64 row, i64 kp, i64 k) { return row * kp * 4 + (k >> 5) * TILE_KB + (k & 31) * 2; }
+__device__ inline float split_load(const u8* p) { return (float)*(const f16*)p + (float)*(const f16*)(p + 32); }
+__device__ inline i64 split_off(i64 row, i64 kp, i64 k) { return row * kp * 4 + (k >> 4) * TILE_KB + (k & 15) * 2; }
 
 // momentum (in place) and partial sums of squares of the update, in float64: the squares of float32 values can leave float32
 template <class T>
@@ -114,68 +114,106 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     }
 }
 
-// D[m][n] = sum_k P[m][k] Q[n][k] over split operands, 64 x 64 per workgroup, 4 waves of 32 x 32
-__device__ inline void split_product(const u8* P, const u8* Q, i64 m0, i64 n0, int kp, u8* tp, u8* tq, f32x16& acc) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32;
-    const i64 pitch = (i64)kp * 4;
-    for (int k0 = 0; k0 < kp; k0 += 32) {
-        for (int i = 0; i < 2; i++) {
-            const int row = (tid >> 3) + 32 * i, piece = tid & 7;
-            *(u32x4*)(tp + tile_off(row, piece)) = *(const u32x4*)(P + (m0 + row) * pitch + (i64)k0 * 4 + piece * 16);
-            *(u32x4*)(tq + tile_off(row, piece)) = *(const u32x4*)(Q + (n0 + row) * pitch + (i64)k0 * 4 + piece * 16);
-        }
-        __syncthreads();
-        for (int ks = 0; ks < 2; ks++) {
-            const int piece = 2 * ks + (lane >> 5), ra = wm + (lane & 31), rb = wn + (lane & 31);
-            const f16x8 ah = *(const f16x8*)(tp + tile_off(ra, piece)), al = *(const f16x8*)(tp + tile_off(ra, piece + 4));
-            const f16x8 bh = *(const f16x8*)(tq + tile_off(rb, piece)), bl = *(const f16x8*)(tq + tile_off(rb, piece + 4));
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
-        }
-        __syncthreads();
+typedef f16 f16x2 __attribute__((ext_vector_type(2)));
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+// two neighbouring values of a row (the first one at an even place)
+__device__ inline void split_store2(u8* p, float v0, float v1) {
+    const f16x2 hi = {(f16)v0, (f16)v1}, lo = {(f16)(v0 - (float)hi[0]), (f16)(v1 - (float)hi[1])};
+    *(f16x2*)p = hi;
+    *(f16x2*)(p + 32) = lo;
+}
+// four, the first one at a multiple of four
+__device__ inline void split_store4(u8* p, const float* v) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        hi[e] = (f16)v[e];
+        lo[e] = (f16)(v[e] - (float)hi[e]);
     }
+    *(f16x4*)p = hi;
+    *(f16x4*)(p + 32) = lo;
 }
 
 enum { GRAM = 0, POLY = 1, STEP = 2, LAST = 3 };
+using OTile128 = TileShape<128, 128, 2, 2, 4>;
+using OTile64 = TileShape<64, 64, 2, 2, 4>;
 
-template <int MODE, class T>
-__global__ __launch_bounds__(256) void k_ortho_product(Jobs js, Hyper h, int cur) {
-    __shared__ __attribute__((aligned(16))) u8 tp[OT * TILE_KB], tq[OT * TILE_KB];
-    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// rows and columns of a launch's result (padded)
+__host__ __device__ inline void product_dims(int mode, const Job& J, int& rows, int& cols) {
+    const bool flip = J.rows > J.cols;
+    rows = mode == GRAM || mode == POLY ? J.sp : (mode == STEP || flip ? J.lp : J.sp);
+    cols = mode == LAST && !flip ? J.lp : J.sp;
+}
+
+// GRAM: A = X X^T     POLY: B = a I + b A + c A A^T     STEP: T <- T B (and X)     LAST: the output, in its own orientation
+template <int MODE, class S, class T>
+__global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur) {
+    extern __shared__ __attribute__((aligned(128))) u8 lds[];
+    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Job& J = js.j[ji];
-    const int tl = blockIdx.x - js.first[ji];
     const bool flip = J.rows > J.cols;
     const u8 *P, *Q;
-    int kp, nt;
-    if (MODE == GRAM) { P = Q = J.x; kp = J.lp; nt = J.sp / OT; }
-    else if (MODE == POLY) { P = Q = J.a; kp = J.sp; nt = J.sp / OT; }
-    else if (MODE == STEP || flip) { P = J.t[cur]; Q = J.b; kp = J.sp; nt = J.sp / OT; }
-    else { P = J.b; Q = J.t[cur]; kp = J.sp; nt = J.lp / OT; }   // the output's own orientation
-    const i64 m0 = (i64)(tl / nt) * OT, n0 = (i64)(tl % nt) * OT;
-    f32x16 acc = {};
-    split_product(P, Q, m0, n0, kp, tp, tq, acc);
-    const i64 n = n0 + (wave & 1) * 32 + (lane & 31);
-    for (int r = 0; r < 16; r++) {
-        const i64 m = m0 + (wave >> 1) * 32 + acc_row(r, lane);
-        if (MODE == GRAM) {
-            split_store(J.a + split_off(m, J.sp, n), acc[r] * 0x1p-16f);
-        } else if (MODE == POLY) {
-            const float A = split_load(J.a + split_off(m, J.sp, n)) * 0x1p-12f;
-            const float B = h.c * (acc[r] * 0x1p-24f) + h.b * A + (m == n ? h.a : 0.0f);
-            split_store(J.b + split_off(m, J.sp, n), B * 0x1p11f);
-        } else if (MODE == STEP) {
-            const float v = acc[r] * 0x1p-11f;
-            split_store(J.t[cur ^ 1] + split_off(m, J.sp, n), v);
-            split_store(J.x + split_off(n, J.lp, m), v);
-        } else if (m < J.rows && n < J.cols) {
-            float v = acc[r] * 0x1p-25f;
-            T* w = (T*)J.w + m * J.cols + n;
-            if (h.update) v = to_f32(*w) * h.decay - v * (h.lr * J.kappa);
-            *w = from_f32<T>(v);
+    int kp, rows, cols;
+    product_dims(MODE, J, rows, cols);
+    if (MODE == GRAM) { P = Q = J.x; kp = J.lp; }
+    else if (MODE == POLY) { P = Q = J.a; kp = J.sp; }
+    else if (MODE == STEP || flip) { P = J.t[cur]; Q = J.b; kp = J.sp; }
+    else { P = J.b; Q = J.t[cur]; kp = J.sp; }
+    u32 tm, tn;
+    tile_place(blockIdx.x - js.first[ji], (rows + S::BM - 1) / S::BM, (cols + S::BN - 1) / S::BN, tm, tn);
+    const i64 m0 = (i64)tm * S::BM, n0 = (i64)tn * S::BN;
+    const u32 pitch = (u32)kp * 4;
+    const u32 mrows = (u32)(rows - m0 < S::BM ? rows - m0 : S::BM), nrows = (u32)(cols - n0 < S::BN ? cols - n0 : S::BN);
+    const TileSrc<false> p(P + m0 * pitch, pitch, mrows * pitch, lane);
+    const TileSrc<S::PAIRS> q(Q + n0 * pitch, pitch, nrows * pitch, lane);
+    f32x16 acc[S::FM][S::FN] = {};
+    tile_product<KindSplit, S>(KindSplit(), p, q, 0, pitch, lds, wave, lane, acc);
+    // lane: columns n and (PAIRS) n + 1, rows in groups of 4
+    const i64 n = n0 + wave % S::WN * (S::FN * 32) + (S::PAIRS ? 2 * (lane & 31) : lane & 31);
+    if (n >= cols) return;
+#pragma unroll
+    for (int i = 0; i < S::FM; i++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const i64 m = m0 + wave / S::WN * (S::FM * 32) + 32 * i + acc_row(4 * g, lane);
+            if (m >= rows) continue;                       // rows and cols are multiples of 64: whole groups, whole pairs
+            float v[S::FN][4];
+#pragma unroll
+            for (int j = 0; j < S::FN; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[j][e] = acc[i][j][4 * g + e];
+                    if (MODE == GRAM) v[j][e] *= 0x1p-16f;
+                    if (MODE == STEP) v[j][e] *= 0x1p-11f;
+                    if (MODE == POLY) {
+                        const float A = split_load(J.a + split_off(m + e, J.sp, n + j)) * 0x1p-12f;
+                        v[j][e] = (h.c * (v[j][e] * 0x1p-24f) + h.b * A + (m + e == n + j ? h.a : 0.0f)) * 0x1p11f;
+                    }
+                }
+            if (MODE != LAST) {
+                u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : J.t[cur ^ 1];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    u8* d = out + split_off(m + e, J.sp, n);
+                    if (S::PAIRS) split_store2(d, v[0][e], v[S::FN - 1][e]);
+                    else split_store(d, v[0][e]);
+                }
+                if (MODE == STEP)
+#pragma unroll
+                    for (int j = 0; j < S::FN; j++) split_store4(J.x + split_off(n + j, J.lp, m), v[j]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+#pragma unroll
+                    for (int j = 0; j < S::FN; j++) {
+                        if (m + e >= J.rows || n + j >= J.cols) continue;
+                        float o = v[j][e] * 0x1p-25f;
+                        T* w = (T*)J.w + (m + e) * J.cols + n + j;
+                        if (h.update) o = to_f32(*w) * h.decay - o * (h.lr * J.kappa);
+                        *w = from_f32<T>(o);
+                    }
+            }
         }
-    }
 }
 
 // ---------------------------------------------------------------------------------------------------- host side
@@ -226,6 +264,14 @@ static bool coeffs_ok(int steps, const double* k) {
     return true;
 }
 
+template <int V>
+struct Int {
+    static constexpr int value = V;
+};
+template <class T>
+struct Type {
+    typedef T type;
+};
 template <class F>
 static void each_first(Jobs& js, F blocks) {
     js.first[0] = 0;
@@ -237,16 +283,33 @@ static int run_jobs(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t 
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
+    auto launch = [&](auto mode, auto t, int cur) {
+        constexpr int MODE = decltype(mode)::value;
+        typedef typename decltype(t)::type T;
+        auto blocks = [&](int edge) {
+            each_first(js, [&](const Job& J) {
+                int rows, cols;
+                product_dims(MODE, J, rows, cols);
+                return (i64)((rows + edge - 1) / edge) * ((cols + edge - 1) / edge);
+            });
+            return js.first[js.n];
+        };
+        // the larger tile reads half as much per product; it needs enough tiles to fill the chip
+        if (blocks(128) >= 160) {
+            k_ortho_product<MODE, OTile128, T><<<dim3(js.first[js.n]), dim3(OTile128::THREADS), OTile128::LDS, st>>>(js, h, cur);
+        } else {
+            const u32 n = (u32)blocks(64);
+            k_ortho_product<MODE, OTile64, T><<<dim3(n), dim3(OTile64::THREADS), OTile64::LDS, st>>>(js, h, cur);
+        }
+    };
     int cur = 0;
     for (int it = 0; it < steps; it++) {
-        each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.sp / OT); });
-        k_ortho_product<GRAM, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
-        k_ortho_product<POLY, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
-        each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
+        launch(Int<GRAM>(), Type<float>(), cur);
+        launch(Int<POLY>(), Type<float>(), cur);
         if (it + 1 < steps) {
-            k_ortho_product<STEP, float><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur);
+            launch(Int<STEP>(), Type<float>(), cur);
         } else {
-            AZ_DISPATCH_DTYPE(dtype, k_ortho_product<LAST, T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h, cur));
+            AZ_DISPATCH_DTYPE(dtype, launch(Int<LAST>(), Type<T>(), cur));
         }
         cur ^= 1;
     }

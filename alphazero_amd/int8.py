@@ -6,7 +6,7 @@ import torch
 
 from . import _abi
 from ._abi import AzError, check, lib
-from ._tensors import DTYPES, address, need, no_grad, rows_of, same_device, stream_of, workspace
+from ._tensors import DTYPES, no_grad, rows_of, same_device, stream_of, vector, workspace
 
 MAX_K = 131071   # the longest sum of products of two 8-bit integers that int32 holds
 
@@ -16,44 +16,56 @@ def quantize_rows(x, index=None):
 
     x: [rows, cols] float32 / float16 / bfloat16 with contiguous rows.  index: int32 [rows, taps] -- row r of q is then
     x[index[r, 0]], x[index[r, 1]], ... one after the other under one scale; an index outside x stands for zeros."""
-    need(x.dtype in DTYPES, "quantize_rows: x must be float32, float16 or bfloat16")
+    dtype = DTYPES.get(x.dtype)
+    if dtype is None:
+        raise AzError("quantize_rows: x must be float32, float16 or bfloat16")
     no_grad("quantize_rows", x)
-    ld = rows_of(x, "quantize_rows: x")
+    n_src, cols, ld = rows_of(x, "quantize_rows", "x")
     dev = same_device("quantize_rows", x, index)
-    n_src, cols = x.shape
-    need(cols >= 1, "quantize_rows: x has no columns")
-    rows, taps = n_src, 1
-    if index is not None:
-        need(index.dtype == torch.int32 and index.dim() == 2 and index.is_contiguous() and index.shape[1] >= 1,
-             "quantize_rows: index must be a contiguous int32 [rows, taps]")
-        rows, taps = index.shape
+    if cols < 1:
+        raise AzError("quantize_rows: x has no columns")
+    if index is None:
+        rows, taps, where = n_src, 1, None
+    else:
+        if index.dtype is not torch.int32 or index.dim() != 2 or not index.is_contiguous() or index.shape[1] < 1:
+            raise AzError("quantize_rows: index must be a contiguous int32 [rows, taps]")
+        (rows, taps), where = index.shape, index.data_ptr()
     q = torch.empty((rows, taps * cols), dtype=torch.int8, device=x.device)
     scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    check(lib().az_i8_quantize_dev(dev, DTYPES[x.dtype], rows, cols, address(x), ld, n_src, address(index), taps, address(q),
-                                   taps * cols, address(scale), stream_of(dev)))
+    check(lib().az_i8_quantize_dev(dev, dtype, rows, cols, x.data_ptr(), ld, n_src, where, taps, q.data_ptr(), taps * cols,
+                                   scale.data_ptr(), stream_of(dev)))
     return q, scale
 
 
 def _layer(what, m, k, w, w_scale, bias, residual, act, dtype, out):
-    need(w.dtype == torch.int8, "%s: w must be int8" % what)
-    ld_w = rows_of(w, "%s: w" % what)
-    n = w.shape[0]
-    need(w.shape[1] == k, "%s: x has %d columns, w has %d" % (what, k, w.shape[1]))
-    need(1 <= k <= MAX_K, "%s: between 1 and %d columns" % (what, MAX_K))
-    need(dtype in DTYPES, "%s: dtype must be float32, float16 or bfloat16" % what)
-    need(act in _abi.ACTS, "%s: act must be one of %s" % (what, ", ".join(sorted(_abi.ACTS))))
-    for t, size, name in ((w_scale, n, "w_scale"), (bias, n, "bias")):
-        need(t is None or (t.dtype == torch.float32 and tuple(t.shape) == (size,) and t.is_contiguous()),
-             "%s: %s must be a contiguous float32 [%d]" % (what, name, size))
-    ld_res = 0
+    """the arguments that matmul and linear share, checked: n, the output, and the tail of the C call up to ld_y"""
+    if w.dtype is not torch.int8:
+        raise AzError("%s: w must be int8" % what)
+    n, k_w, ld_w = rows_of(w, what, "w")
+    if k_w != k:
+        raise AzError("%s: x has %d columns, w has %d" % (what, k, k_w))
+    if not 1 <= k <= MAX_K:
+        raise AzError("%s: between 1 and %d columns" % (what, MAX_K))
+    code, fn = DTYPES.get(dtype), _abi.ACTS.get(act)
+    if code is None:
+        raise AzError("%s: dtype must be float32, float16 or bfloat16" % what)
+    if fn is None:
+        raise AzError("%s: act must be one of %s" % (what, ", ".join(sorted(_abi.ACTS))))
+    ws = vector(w_scale, n, what, "w_scale")
+    b = None if bias is None else vector(bias, n, what, "bias")
+    res, ld_res = None, 0
     if residual is not None:
-        need(residual.dtype == dtype and tuple(residual.shape) == (m, n), "%s: residual must be [%d, %d] of the output's dtype"
-             % (what, m, n))
-        ld_res = rows_of(residual, "%s: residual" % what)
+        r_m, r_n, ld_res = rows_of(residual, what, "residual")
+        if residual.dtype is not dtype or r_m != m or r_n != n:
+            raise AzError("%s: residual must be [%d, %d] of the output's dtype" % (what, m, n))
+        res = residual.data_ptr()
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=w.device)
-    need(out.dtype == dtype and tuple(out.shape) == (m, n), "%s: out must be [%d, %d] of the output's dtype" % (what, m, n))
-    return n, ld_w, ld_res, out, rows_of(out, "%s: out" % what)
+        out, ld_y = torch.empty((m, n), dtype=dtype, device=w.device), n
+    else:
+        o_m, o_n, ld_y = rows_of(out, what, "out")
+        if out.dtype is not dtype or o_m != m or o_n != n:
+            raise AzError("%s: out must be [%d, %d] of the output's dtype" % (what, m, n))
+    return n, w.data_ptr(), ld_w, out, (ws, b, res, ld_res, fn, code, out.data_ptr(), ld_y)
 
 
 def matmul(q, scale, w, w_scale, bias=None, residual=None, act="none", dtype=torch.float32, out=None):
@@ -61,35 +73,32 @@ def matmul(q, scale, w, w_scale, bias=None, residual=None, act="none", dtype=tor
 
     q int8 [m, k], w int8 [n, k] with contiguous rows; scale [m], w_scale [n], bias [n] float32; residual [m, n] of `dtype`
     (may be `out` itself); act: "none", "relu" or "silu".  Integer sums are exact, the rest is float32, rounded once."""
-    need(q.dtype == torch.int8, "matmul: q must be int8")
-    ld_q = rows_of(q, "matmul: q")
-    m, k = q.shape
-    need(scale.dtype == torch.float32 and tuple(scale.shape) == (m,) and scale.is_contiguous(),
-         "matmul: scale must be a contiguous float32 [%d]" % m)
+    if q.dtype is not torch.int8:
+        raise AzError("matmul: q must be int8")
+    m, k, ld_q = rows_of(q, "matmul", "q")
     no_grad("matmul", scale, w_scale, bias, residual)
     dev = same_device("matmul", q, scale, w, w_scale, bias, residual, out)
-    n, ld_w, ld_res, out, ld_y = _layer("matmul", m, k, w, w_scale, bias, residual, act, dtype, out)
-    L = lib()
-    nws = L.az_i8_matmul_ws(m, n, k)
-    ws = workspace(nws, q.device)
-    check(L.az_i8_matmul_dev(dev, m, n, k, address(q), ld_q, address(scale), address(w), ld_w, address(w_scale), address(bias),
-                             address(residual), ld_res, _abi.ACTS[act], DTYPES[dtype], address(out), ld_y, address(ws),
-                             ws.numel(), stream_of(dev)))
+    s = vector(scale, m, "matmul", "scale")
+    n, wp, ld_w, out, tail = _layer("matmul", m, k, w, w_scale, bias, residual, act, dtype, out)
+    L, qp = lib(), q.data_ptr()
+    nws = L.az_i8_matmul_ws(m, n, k, qp, ld_q, wp, ld_w)
+    ws, wsp = workspace(nws, q)
+    check(L.az_i8_matmul_dev(dev, m, n, k, qp, ld_q, s, wp, ld_w, *tail, wsp, nws, stream_of(dev)))
     return out
 
 
 def linear(x, w, w_scale, bias=None, residual=None, act="none", out=None):
     """quantize_rows(x), then matmul with the result; the output has x's dtype."""
-    need(x.dtype in DTYPES, "linear: x must be float32, float16 or bfloat16")
+    if x.dtype not in DTYPES:
+        raise AzError("linear: x must be float32, float16 or bfloat16")
+    m, k, ld_x = rows_of(x, "linear", "x")
     no_grad("linear", x, w_scale, bias, residual)
-    ld_x = rows_of(x, "linear: x")
-    m, k = x.shape
     dev = same_device("linear", x, w, w_scale, bias, residual, out)
-    n, ld_w, ld_res, out, ld_y = _layer("linear", m, k, w, w_scale, bias, residual, act, x.dtype, out)
-    need(out.data_ptr() != x.data_ptr() or m * n == 0, "linear: out must not be x")
-    L = lib()
-    ws = workspace(L.az_i8_linear_ws(m, n, k), x.device)
-    check(L.az_i8_linear_dev(dev, m, n, k, address(x), ld_x, address(w), ld_w, address(w_scale), address(bias),
-                             address(residual), ld_res, _abi.ACTS[act], DTYPES[x.dtype], address(out), ld_y, address(ws),
-                             ws.numel(), stream_of(dev)))
+    n, wp, ld_w, out, tail = _layer("linear", m, k, w, w_scale, bias, residual, act, x.dtype, out)
+    L, xp = lib(), x.data_ptr()
+    if m * n > 0 and out.data_ptr() == xp:
+        raise AzError("linear: out must not be x")
+    nws = L.az_i8_linear_ws(m, n, k, wp, ld_w)
+    ws, wsp = workspace(nws, x)
+    check(L.az_i8_linear_dev(dev, m, n, k, xp, ld_x, wp, ld_w, *tail, wsp, nws, stream_of(dev)))
     return out

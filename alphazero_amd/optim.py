@@ -7,38 +7,38 @@ import torch
 
 from . import _abi
 from ._abi import AzError, check, lib
-from ._tensors import DTYPES, address, need, no_grad, same_device, stream_of, workspace
+from ._tensors import DTYPES, no_grad, same_device, stream_of, workspace
 
 COEFFS = (3.4445, -4.7750, 2.0315)
 
 
 def _coeffs(coeffs):
-    need(len(coeffs) == 3, "coeffs must be (a, b, c)")
-    return (C.c_double * 3)(*[float(c) for c in coeffs])
+    if len(coeffs) != 3:
+        raise AzError("coeffs must be (a, b, c)")
+    return (C.c_double * 3)(*coeffs)
 
 
 def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, out=None):
     """The orthogonalisation of every matrix g[..., rows, cols] by `steps` Newton-Schulz products (float32-accurate):
     X = G / (||G||_F + eps), X <- a X + (b A + c A^2) X with A = X X^T.  out: a contiguous tensor like g (may be g)."""
-    need(g.dtype in DTYPES, "orthogonalize: g must be float32, float16 or bfloat16")
-    need(g.dim() >= 2, "orthogonalize: g must have at least two dimensions")
+    if g.dtype not in DTYPES or g.dim() < 2:
+        raise AzError("orthogonalize: g must be float32, float16 or bfloat16 of at least two dimensions")
     no_grad("orthogonalize", g)
     dev = same_device("orthogonalize", g, out)
     rows, cols = g.shape[-2:]
-    batch = 1
-    for d in g.shape[:-2]:
-        batch *= d
     if out is None:
         out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    need(out.dtype == g.dtype and out.shape == g.shape and out.is_contiguous(),
-         "orthogonalize: out must be contiguous, of g's shape and dtype")
-    if batch * rows * cols == 0:
+    elif out.dtype is not g.dtype or out.shape != g.shape or not out.is_contiguous():
+        raise AzError("orthogonalize: out must be contiguous, of g's shape and dtype")
+    if g.numel() == 0:
         return out
+    batch = g.numel() // (rows * cols)
     g = g.contiguous()
     L = lib()
-    ws = workspace(L.az_orthogonalize_ws(batch, rows, cols), g.device)
-    check(L.az_orthogonalize_dev(dev, DTYPES[g.dtype], batch, rows, cols, address(g), address(out), int(steps), _coeffs(coeffs),
-                                 float(eps), address(ws), ws.numel(), stream_of(dev)))
+    nws = L.az_orthogonalize_ws(batch, rows, cols)
+    ws, wsp = workspace(nws, g)
+    check(L.az_orthogonalize_dev(dev, DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, _coeffs(coeffs),
+                                 eps, wsp, nws, stream_of(dev)))
     return out
 
 
@@ -49,25 +49,31 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
     weights, grads: lists of contiguous tensors [rows, ...] of one dtype, seen as [rows, rest]; momenta: float32 of the same
-    shapes.  No tensor may appear twice among weights and momenta."""
-    weights, grads, momenta = list(weights), list(grads), list(momenta)
-    need(len(weights) == len(grads) == len(momenta), "muon_step: as many gradients and momenta as weights")
-    if not weights:
+    shapes.  No weight or momentum may overlap another one or a gradient."""
+    n = len(weights)
+    if len(grads) != n or len(momenta) != n:
+        raise AzError("muon_step: as many gradients and momenta as weights")
+    if n == 0:
         return
     dt = weights[0].dtype
-    need(dt in DTYPES, "muon_step: weights must be float32, float16 or bfloat16")
+    if dt not in DTYPES:
+        raise AzError("muon_step: weights must be float32, float16 or bfloat16")
     dev = same_device("muon_step", *weights, *grads, *momenta)
-    items = (_abi.az_muon_item * len(weights))()
+    items = (_abi.az_muon_item * n)()
     for it, w, g, m in zip(items, weights, grads, momenta):
-        need(w.dim() >= 2 and w.numel() > 0, "muon_step: weights must have at least two dimensions and no empty one")
-        need(w.dtype == dt and g.dtype == dt and m.dtype == torch.float32,
-             "muon_step: weights and gradients of one dtype, momenta of float32")
-        need(w.shape == g.shape == m.shape, "muon_step: weights, gradients and momenta must have the same shapes")
-        need(w.is_contiguous() and g.is_contiguous() and m.is_contiguous(), "muon_step: tensors must be contiguous")
-        it.w_dev, it.g_dev, it.m_dev = address(w), address(g), address(m)
-        it.rows, it.cols = w.shape[0], w.numel() // w.shape[0]
+        if w.dim() < 2 or w.numel() == 0:
+            raise AzError("muon_step: weights must have at least two dimensions and no empty one")
+        if w.dtype is not dt or g.dtype is not dt or m.dtype is not torch.float32:
+            raise AzError("muon_step: weights and gradients of one dtype, momenta of float32")
+        if w.shape != g.shape or w.shape != m.shape:
+            raise AzError("muon_step: weights, gradients and momenta must have the same shapes")
+        if not (w.is_contiguous() and g.is_contiguous() and m.is_contiguous()):
+            raise AzError("muon_step: tensors must be contiguous")
+        it.w_dev, it.g_dev, it.m_dev = w.data_ptr(), g.data_ptr(), m.data_ptr()
+        it.rows = rows = w.shape[0]
+        it.cols = w.numel() // rows
     L = lib()
-    ws = workspace(L.az_muon_step_ws(items, len(weights)), weights[0].device)
-    check(L.az_muon_step_dev(dev, DTYPES[dt], items, len(weights), float(lr), float(momentum), 1 if nesterov else 0,
-                             float(weight_decay), int(steps), _coeffs(coeffs), float(eps), address(ws), ws.numel(),
-                             stream_of(dev)))
+    nws = L.az_muon_step_ws(items, n)
+    ws, wsp = workspace(nws, weights[0])
+    check(L.az_muon_step_dev(dev, DTYPES[dt], items, n, lr, momentum, 1 if nesterov else 0, weight_decay, steps, _coeffs(coeffs),
+                             eps, wsp, nws, stream_of(dev)))

@@ -315,13 +315,13 @@ int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const 
 /* y[m][n] = act(q_scale[m] * w_scale[n] * sum_k q[m][k] w[n][k] + bias[n] + residual[m][n]), integer sums exact, the rest
  * in float32, rounded once to `dtype` (of y and residual).  bias and residual may be NULL; residual may be y itself.
  * ld_*: elements from row to row.  k <= 131071 (above that a sum could leave int32). */
-size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k);
+size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k, const int8_t *q_dev, int64_t ld_q, const int8_t *w_dev, int64_t ld_w);
 int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t *q_dev, int64_t ld_q,
                      const float *q_scale_dev, const int8_t *w_dev, int64_t ld_w, const float *w_scale_dev,
                      const float *bias_dev, const void *residual_dev, int64_t ld_res, int act, int dtype, void *y_dev,
                      int64_t ld_y, void *ws_dev, size_t ws_bytes, void *stream);
 /* az_i8_quantize_dev followed by az_i8_matmul_dev on rows x[m][k] of `dtype`, ld_x elements apart. */
-size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k);
+size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k, const int8_t *w_dev, int64_t ld_w);
 int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void *x_dev, int64_t ld_x, const int8_t *w_dev,
                      int64_t ld_w, const float *w_scale_dev, const float *bias_dev, const void *residual_dev,
                      int64_t ld_res, int act, int dtype, void *y_dev, int64_t ld_y, void *ws_dev, size_t ws_bytes,
