@@ -130,13 +130,13 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
         const i64 r = rows < most ? rows : most;
         return (u32)((r - 1) * ld + k);
     };
-    const TileSrc<false> a(p.q + m0 * p.ld_q, (u32)p.ld_q, span(p.m - m0, S::BM, p.ld_q, p.k), lane);
-    const TileSrc<S::PAIRS> b(p.w + n0 * p.ld_w, (u32)p.ld_w, span(p.n - n0, S::BN, p.ld_w, p.k), lane);
-    const u32 k0 = blockIdx.y * steps_per_split * TILE_KB;
-    u32 kend = k0 + steps_per_split * TILE_KB;
+    const TileSrc<false> a(p.q + m0 * p.ld_q, TILE_KB, (u32)p.ld_q, span(p.m - m0, S::BM, p.ld_q, p.k), lane);
+    const TileSrc<S::PAIRS> b(p.w + n0 * p.ld_w, TILE_KB, (u32)p.ld_w, span(p.n - n0, S::BN, p.ld_w, p.k), lane);
+    const u32 first = blockIdx.y * steps_per_split;
+    u32 kend = (first + steps_per_split) * TILE_KB;
     kend = kend < (u32)p.k ? kend : (u32)p.k;
     i32x16 acc[S::FM][S::FN] = {};
-    tile_product<KindI8, S>(KindI8(), a, b, k0, kend, lds, wave, lane, acc);
+    tile_product<KindI8, S>(KindI8(), a, b, first, kend, lds, wave, lane, acc);
     // scales of the tile's rows and columns through LDS (its tiles have been read)
     float *sm = (float*)lds, *sn = sm + S::BM, *bn = sn + S::BN;
     for (int t = threadIdx.x; t < S::BM; t += S::THREADS) sm[t] = p.qs[m0 + t < p.m ? m0 + t : p.m - 1];
@@ -146,45 +146,50 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
         bn[t] = p.bias ? p.bias[n] : 0.0f;
     }
     __syncthreads();
-    const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32), c = S::PAIRS ? 2 * (lane & 31) : lane & 31;
-    const i64 n = n0 + wn + c;
-    const float s0 = sn[wn + c], b0 = bn[wn + c], s1 = S::PAIRS ? sn[wn + c + 1] : 0, b1 = S::PAIRS ? bn[wn + c + 1] : 0;
-    if (n >= p.n) return;
-    const bool two = S::PAIRS && n + 1 < p.n;
+    const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32);
+    constexpr int W = S::PAIRS ? 2 : 1;   // neighbouring columns a lane holds
     if (part) part += (i64)blockIdx.y * p.m * p.n;
 #pragma unroll
-    for (int i = 0; i < S::FM; i++)
+    for (int j = 0; j < S::FN; j += W) {
+        const int c = wn + 32 * j + W * (lane & 31);
+        const i64 n = n0 + c;
+        const float s0 = sn[c], b0 = bn[c], s1 = sn[c + W - 1], b1 = bn[c + W - 1];
+        const bool two = W == 2 && n + 1 < p.n;
+        if (n >= p.n) continue;
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const int row = wm + 32 * i + acc_row(4 * g, lane);
-            const f32x4 s4 = *(const f32x4*)(sm + row);
+        for (int i = 0; i < S::FM; i++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const i64 m = m0 + row + e;
-                if (m >= p.m) break;
-                const int q0 = acc[i][0][4 * g + e], q1 = acc[i][S::FN - 1][4 * g + e];
-                if (part) {
-                    part[m * p.n + n] = q0;
-                    if (two) part[m * p.n + n + 1] = q1;
-                    continue;
-                }
-                float v0 = (float)q0 * s4[e] * s0 + b0, v1 = (float)q1 * s4[e] * s1 + b1;
-                T* y = (T*)p.y + m * p.ld_y + n;
-                if (p.res) {
-                    const T* r = (const T*)p.res + m * p.ld_res + n;
-                    v0 += to_f32(r[0]);
-                    if (two) v1 += to_f32(r[1]);
-                }
-                v0 = activate(v0, p.act);
-                if (S::PAIRS && two && p.pair_store) {
-                    struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
-                    *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate(v1, p.act))};
-                } else {
-                    y[0] = from_f32<T>(v0);
-                    if (two) y[1] = from_f32<T>(activate(v1, p.act));
+            for (int g = 0; g < 4; g++) {
+                const int row = wm + 32 * i + acc_row(4 * g, lane);
+                const f32x4 s4 = *(const f32x4*)(sm + row);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const i64 m = m0 + row + e;
+                    if (m >= p.m) break;
+                    const int q0 = acc[i][j][4 * g + e], q1 = acc[i][j + W - 1][4 * g + e];
+                    if (part) {
+                        part[m * p.n + n] = q0;
+                        if (two) part[m * p.n + n + 1] = q1;
+                        continue;
+                    }
+                    float v0 = (float)q0 * s4[e] * s0 + b0, v1 = (float)q1 * s4[e] * s1 + b1;
+                    T* y = (T*)p.y + m * p.ld_y + n;
+                    if (p.res) {
+                        const T* r = (const T*)p.res + m * p.ld_res + n;
+                        v0 += to_f32(r[0]);
+                        if (two) v1 += to_f32(r[1]);
+                    }
+                    v0 = activate(v0, p.act);
+                    if (two && p.pair_store) {
+                        struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
+                        *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate(v1, p.act))};
+                    } else {
+                        y[0] = from_f32<T>(v0);
+                        if (two) y[1] = from_f32<T>(activate(v1, p.act));
+                    }
                 }
             }
-        }
+    }
 }
 template <class T>
 __global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __restrict__ part) {

@@ -29,7 +29,7 @@ struct Job {
     i32 rows, cols, s, l, sp, lp, n_part;
     float kappa;
     double* part;
-    u8 *x, *t[2], *a, *b;   // split operands; a row of k values is k / 16 blocks of 64 bytes (16 hi, 16 lo)
+    u8 *x, *t[2], *a, *b;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
 };
 struct Jobs {
     Job j[MAX_JOBS];
@@ -59,8 +59,7 @@ __device__ inline void split_store(u8* p, float v) {   // p: the high half's pla
     *(f16*)p = hi;
     *(f16*)(p + 32) = (f16)(v - (float)hi);
 }
-__device__ inline float split_load(const u8* p) { return (float)*(const f16*)p + (float)*(const f16*)(p + 32); }
-__device__ inline i64 split_off(i64 row, i64 kp, i64 k) { return row * kp * 4 + (k >> 4) * TILE_KB + (k & 15) * 2; }
+__device__ inline i64 split_off(i64 row, i64 rows, i64 k) { return ((k >> 4) * rows + row) * TILE_KB + (k & 15) * 2; }
 
 // momentum (in place) and partial sums of squares of the update, in float64: the squares of float32 values can leave float32
 template <class T>
@@ -109,34 +108,31 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     __syncthreads();
     for (int e = tid; e < OT * OT; e += 256) {
         const int r = e / OT, c = e % OT;
-        split_store(J.x + split_off(i0 + r, J.lp, j0 + c), tile[r][c]);
-        split_store(J.t[0] + split_off(j0 + r, J.sp, i0 + c), tile[c][r]);
+        split_store(J.x + split_off(i0 + r, J.sp, j0 + c), tile[r][c]);
+        split_store(J.t[0] + split_off(j0 + r, J.lp, i0 + c), tile[c][r]);
     }
 }
 
-typedef f16 f16x2 __attribute__((ext_vector_type(2)));
-typedef f16 f16x4 __attribute__((ext_vector_type(4)));
-// two neighbouring values of a row (the first one at an even place)
-__device__ inline void split_store2(u8* p, float v0, float v1) {
-    const f16x2 hi = {(f16)v0, (f16)v1}, lo = {(f16)(v0 - (float)hi[0]), (f16)(v1 - (float)hi[1])};
-    *(f16x2*)p = hi;
-    *(f16x2*)(p + 32) = lo;
-}
-// four, the first one at a multiple of four
-__device__ inline void split_store4(u8* p, const float* v) {
-    f16x4 hi, lo;
+// eight values of a row from a multiple of eight on: their halves, 16 bytes each
+__device__ inline void split_store8(u8* p, const float (&v)[8]) {
+    f16x8 hi, lo;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < 8; e++) {
         hi[e] = (f16)v[e];
         lo[e] = (f16)(v[e] - (float)hi[e]);
     }
-    *(f16x4*)p = hi;
-    *(f16x4*)(p + 32) = lo;
+    *(f16x8*)p = hi;
+    *(f16x8*)(p + 32) = lo;
+}
+__device__ inline void split_load8(const u8* p, float (&v)[8]) {
+    const f16x8 hi = *(const f16x8*)p, lo = *(const f16x8*)(p + 32);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)hi[e] + (float)lo[e];
 }
 
 enum { GRAM = 0, POLY = 1, STEP = 2, LAST = 3 };
-using OTile128 = TileShape<128, 128, 2, 2, 4>;
-using OTile64 = TileShape<64, 64, 2, 2, 4>;
+// GRAM: A = X X^T     POLY: B = a I + b A + c A A^T     STEP: T <- T B (and X)     LAST: the output, in its own orientation
+// A and B are symmetric: their launches compute the tiles that touch the lower triangle and store them twice.
 
 // rows and columns of a launch's result (padded)
 __host__ __device__ inline void product_dims(int mode, const Job& J, int& rows, int& cols) {
@@ -144,14 +140,28 @@ __host__ __device__ inline void product_dims(int mode, const Job& J, int& rows, 
     rows = mode == GRAM || mode == POLY ? J.sp : (mode == STEP || flip ? J.lp : J.sp);
     cols = mode == LAST && !flip ? J.lp : J.sp;
 }
+// tiles of a symmetric launch: tile row i covers rows from bm i on and has the tiles whose first column is not behind its last
+// row: (i + 1) bm / bn of them, but for the last row, which ends with the matrix
+__host__ __device__ inline int symmetric_tiles(int n, int bm, int bn) {
+    const int full = n / bm, per = bm / bn;
+    return per * full * (full + 1) / 2 + (n % bm ? (n + bn - 1) / bn : 0);
+}
 
-// GRAM: A = X X^T     POLY: B = a I + b A + c A A^T     STEP: T <- T B (and X)     LAST: the output, in its own orientation
+// the tile's result passes through LDS as float32, so that rows leave it 16 bytes a lane
+template <class S>
+struct Staged {
+    static constexpr int PITCH = S::BN + 4;   // floats; rows stay 16-byte aligned and start 4 banks apart
+    static constexpr int BYTES = S::BM * PITCH * 4;
+    static constexpr int LDS = BYTES > S::LDS ? BYTES : S::LDS;
+};
+
 template <int MODE, class S, class T>
 __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
-    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ji = find_job(js, blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Job& J = js.j[ji];
     const bool flip = J.rows > J.cols;
+    constexpr bool SYM = MODE == GRAM || MODE == POLY;
     const u8 *P, *Q;
     int kp, rows, cols;
     product_dims(MODE, J, rows, cols);
@@ -160,61 +170,87 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
     else if (MODE == STEP || flip) { P = J.t[cur]; Q = J.b; kp = J.sp; }
     else { P = J.b; Q = J.t[cur]; kp = J.sp; }
     u32 tm, tn;
-    tile_place(blockIdx.x - js.first[ji], (rows + S::BM - 1) / S::BM, (cols + S::BN - 1) / S::BN, tm, tn);
-    const i64 m0 = (i64)tm * S::BM, n0 = (i64)tn * S::BN;
-    const u32 pitch = (u32)kp * 4;
-    const u32 mrows = (u32)(rows - m0 < S::BM ? rows - m0 : S::BM), nrows = (u32)(cols - n0 < S::BN ? cols - n0 : S::BN);
-    const TileSrc<false> p(P + m0 * pitch, pitch, mrows * pitch, lane);
-    const TileSrc<S::PAIRS> q(Q + n0 * pitch, pitch, nrows * pitch, lane);
+    const int block = blockIdx.x - js.first[ji];
+    if (SYM) {
+        constexpr int PER = S::BM / S::BN;
+        tm = (u32)((sqrtf(8.0f * (float)(block / PER) + 1.0f) - 1.0f) * 0.5f);   // the row i with PER i (i + 1) / 2 <= block
+        while (PER * tm * (tm + 1) / 2 > (u32)block) tm--;
+        while (PER * (tm + 1) * (tm + 2) / 2 <= (u32)block) tm++;
+        tn = block - PER * tm * (tm + 1) / 2;
+    } else {
+        tile_place(block, (rows + S::BM - 1) / S::BM, (cols + S::BN - 1) / S::BN, tm, tn);
+    }
+    const int m0 = tm * S::BM, n0 = tn * S::BN;
+    const int mrows = rows - m0 < S::BM ? rows - m0 : S::BM, ncols = cols - n0 < S::BN ? cols - n0 : S::BN;
+    const TileSrc<false> p(P + m0 * TILE_KB, (u64)rows * TILE_KB, TILE_KB, mrows * TILE_KB, lane);
+    const TileSrc<S::PAIRS> q(Q + n0 * TILE_KB, (u64)cols * TILE_KB, TILE_KB, ncols * TILE_KB, lane);
     f32x16 acc[S::FM][S::FN] = {};
-    tile_product<KindSplit, S>(KindSplit(), p, q, 0, pitch, lds, wave, lane, acc);
-    // lane: columns n and (PAIRS) n + 1, rows in groups of 4
-    const i64 n = n0 + wave % S::WN * (S::FN * 32) + (S::PAIRS ? 2 * (lane & 31) : lane & 31);
-    if (n >= cols) return;
+    tile_product<KindSplit, S>(KindSplit(), p, q, 0, kp * 4, lds, wave, lane, acc);
+
+    constexpr int W = S::PAIRS ? 2 : 1, PITCH = Staged<S>::PITCH;
+    constexpr float UNIT = MODE == GRAM ? 0x1p-16f : MODE == POLY ? 0x1p-24f : MODE == STEP ? 0x1p-11f : 0x1p-25f;
+    float* tile = (float*)lds;
 #pragma unroll
     for (int i = 0; i < S::FM; i++)
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const i64 m = m0 + wave / S::WN * (S::FM * 32) + 32 * i + acc_row(4 * g, lane);
-            if (m >= rows) continue;                       // rows and cols are multiples of 64: whole groups, whole pairs
-            float v[S::FN][4];
+        for (int j = 0; j < S::FN; j += W)
 #pragma unroll
-            for (int j = 0; j < S::FN; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    v[j][e] = acc[i][j][4 * g + e];
-                    if (MODE == GRAM) v[j][e] *= 0x1p-16f;
-                    if (MODE == STEP) v[j][e] *= 0x1p-11f;
-                    if (MODE == POLY) {
-                        const float A = split_load(J.a + split_off(m + e, J.sp, n + j)) * 0x1p-12f;
-                        v[j][e] = (h.c * (v[j][e] * 0x1p-24f) + h.b * A + (m + e == n + j ? h.a : 0.0f)) * 0x1p11f;
-                    }
-                }
-            if (MODE != LAST) {
-                u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : J.t[cur ^ 1];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    u8* d = out + split_off(m + e, J.sp, n);
-                    if (S::PAIRS) split_store2(d, v[0][e], v[S::FN - 1][e]);
-                    else split_store(d, v[0][e]);
-                }
-                if (MODE == STEP)
-#pragma unroll
-                    for (int j = 0; j < S::FN; j++) split_store4(J.x + split_off(n + j, J.lp, m), v[j]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int j = 0; j < S::FN; j++) {
-                        if (m + e >= J.rows || n + j >= J.cols) continue;
-                        float o = v[j][e] * 0x1p-25f;
-                        T* w = (T*)J.w + (m + e) * J.cols + n + j;
-                        if (h.update) o = to_f32(*w) * h.decay - o * (h.lr * J.kappa);
-                        *w = from_f32<T>(o);
-                    }
+            for (int r = 0; r < 16; r++) {
+                float* d = tile + (wave / S::WN * (S::FM * 32) + 32 * i + acc_row(r, lane)) * PITCH + wave % S::WN * (S::FN * 32) +
+                           32 * j + W * (lane & 31);
+                d[0] = acc[i][j][r] * UNIT;
+                if (W == 2) d[1] = acc[i][j + W - 1][r] * UNIT;
             }
+    __syncthreads();
+    if (MODE != LAST) {   // mrows and ncols are multiples of 64 here
+        u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : J.t[cur ^ 1];
+        // pairs of lanes store 16 values of a row, 64 bytes; the next pair those of the next row, right behind them
+        for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
+            const int r = u / 2 % S::BM, c = (u % 2 + u / (2 * S::BM) * 2) * 8, m = m0 + r, n = n0 + c;
+            if (r >= mrows || c >= ncols) continue;
+            float v[8];
+            float* d = tile + r * PITCH + c;
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = d[e];
+            if (MODE == POLY) {
+                float A[8];
+                split_load8(J.a + split_off(m, J.sp, n), A);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    v[e] = (h.c * v[e] + h.b * (A[e] * 0x1p-12f) + (m == n + e ? h.a : 0.0f)) * 0x1p11f;
+                    d[e] = v[e];
+                }
+            }
+            split_store8(out + split_off(m, rows, n), v);
         }
+        // transposed: X for STEP, the mirrored tile for A and B.  The tiles across the diagonal cover both sides themselves: a
+        // mirrored value could differ from the computed one in its last bit, and both would be written.
+        if (SYM && n0 + S::BN > m0) return;
+        if (MODE == POLY) __syncthreads();
+        u8* outT = MODE == STEP ? J.x : out;
+        for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
+            const int c = u / 2 % S::BN, r = (u % 2 + u / (2 * S::BN) * 2) * 8;
+            if (r >= mrows || c >= ncols) continue;
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = tile[(r + e) * PITCH + c];
+            split_store8(outT + split_off(n0 + c, cols, m0 + r), v);
+        }
+    } else {
+        for (int u = tid; u < S::BM * S::BN; u += S::THREADS) {
+            const int r = u / S::BN, c = u % S::BN;
+            if (m0 + r >= J.rows || n0 + c >= J.cols) continue;
+            float o = tile[r * PITCH + c];
+            T* w = (T*)J.w + (i64)(m0 + r) * J.cols + n0 + c;
+            if (h.update) o = to_f32(*w) * h.decay - o * (h.lr * J.kappa);
+            *w = from_f32<T>(o);
+        }
+    }
 }
+
+using OTile128 = TileShape<128, 128, 2, 2, 4>;
+using OTile128s = TileShape<128, 64, 2, 2, 4>;   // symmetric results
+using OTile64 = TileShape<64, 64, 2, 2, 4>;
 
 // ---------------------------------------------------------------------------------------------------- host side
 static i64 pad(i64 n) { return (n + OT - 1) / OT * OT; }
@@ -264,18 +300,40 @@ static bool coeffs_ok(int steps, const double* k) {
     return true;
 }
 
-template <int V>
-struct Int {
-    static constexpr int value = V;
-};
-template <class T>
-struct Type {
-    typedef T type;
-};
 template <class F>
 static void each_first(Jobs& js, F blocks) {
     js.first[0] = 0;
     for (int i = 0; i < js.n; i++) js.first[i + 1] = js.first[i] + (i32)blocks(js.j[i]);
+}
+
+template <int MODE, class S>
+static int product_blocks(Jobs& js) {   // fills js.first
+    each_first(js, [](const Job& J) {
+        int rows, cols;
+        product_dims(MODE, J, rows, cols);
+        if (MODE == GRAM || MODE == POLY) return (i64)symmetric_tiles(J.sp, S::BM, S::BN);
+        return (i64)((rows + S::BM - 1) / S::BM) * ((cols + S::BN - 1) / S::BN);
+    });
+    return js.first[js.n];
+}
+template <int MODE, class T>
+static void product(Jobs& js, const Hyper& h, int cur, hipStream_t st) {
+    // the larger tile reads half as much per product; it needs enough tiles to fill the chip
+    if constexpr (MODE == GRAM || MODE == POLY) {
+        const int n = product_blocks<MODE, OTile128s>(js);
+        if (n >= 160) {
+            k_ortho_product<MODE, OTile128s, T><<<dim3((u32)n), dim3(OTile128s::THREADS), Staged<OTile128s>::LDS, st>>>(js, h, cur);
+            return;
+        }
+    } else {
+        const int n = product_blocks<MODE, OTile128>(js);
+        if (n >= 160) {
+            k_ortho_product<MODE, OTile128, T><<<dim3((u32)n), dim3(OTile128::THREADS), Staged<OTile128>::LDS, st>>>(js, h, cur);
+            return;
+        }
+    }
+    const int n = product_blocks<MODE, OTile64>(js);
+    k_ortho_product<MODE, OTile64, T><<<dim3((u32)n), dim3(OTile64::THREADS), Staged<OTile64>::LDS, st>>>(js, h, cur);
 }
 
 static int run_jobs(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
@@ -283,33 +341,14 @@ static int run_jobs(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t 
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
-    auto launch = [&](auto mode, auto t, int cur) {
-        constexpr int MODE = decltype(mode)::value;
-        typedef typename decltype(t)::type T;
-        auto blocks = [&](int edge) {
-            each_first(js, [&](const Job& J) {
-                int rows, cols;
-                product_dims(MODE, J, rows, cols);
-                return (i64)((rows + edge - 1) / edge) * ((cols + edge - 1) / edge);
-            });
-            return js.first[js.n];
-        };
-        // the larger tile reads half as much per product; it needs enough tiles to fill the chip
-        if (blocks(128) >= 160) {
-            k_ortho_product<MODE, OTile128, T><<<dim3(js.first[js.n]), dim3(OTile128::THREADS), OTile128::LDS, st>>>(js, h, cur);
-        } else {
-            const u32 n = (u32)blocks(64);
-            k_ortho_product<MODE, OTile64, T><<<dim3(n), dim3(OTile64::THREADS), OTile64::LDS, st>>>(js, h, cur);
-        }
-    };
     int cur = 0;
     for (int it = 0; it < steps; it++) {
-        launch(Int<GRAM>(), Type<float>(), cur);
-        launch(Int<POLY>(), Type<float>(), cur);
+        product<GRAM, float>(js, h, cur, st);
+        product<POLY, float>(js, h, cur, st);
         if (it + 1 < steps) {
-            launch(Int<STEP>(), Type<float>(), cur);
+            product<STEP, float>(js, h, cur, st);
         } else {
-            AZ_DISPATCH_DTYPE(dtype, launch(Int<LAST>(), Type<T>(), cur));
+            AZ_DISPATCH_DTYPE(dtype, product<LAST, T>(js, h, cur, st));
         }
         cur ^= 1;
     }

@@ -20,15 +20,19 @@ __device__ inline int acc_row(int r, int lane) { return 8 * (r >> 2) + 4 * (lane
 
 typedef __attribute__((address_space(3))) void lds_void;
 
-// one operand: rows from `base` on, `ld` bytes apart; reads behind `bytes` give zeros
+// one operand: rows `ld` bytes apart, a step's 64 bytes of them `kstep` bytes behind those of the step before.  Rows of the caller
+// (int8): ld is the row, kstep 64.  Operands of our own are kept in panels, a step's 64 bytes of all rows together: ld is 64 and
+// a step's tile one run of memory (rows a power of two apart crowd into a few channels of L2).
+// Reads behind `bytes` from a step's first row on give zeros.
 // PAIRS: of every 64 rows the even ones come first, then the odd ones.  A wave with two blocks of 32 columns then holds columns
 // 2 c and 2 c + 1 in lane c, and stores them together.
 template <bool PAIRS>
 struct TileSrc {
-    __amdgpu_buffer_rsrc_t rsrc;
-    u32 ld, voff, piece;   // this lane's row and piece inside a group of 16 rows
-    __device__ TileSrc(const void* base, u32 ld_, u32 bytes, int lane) : ld(ld_) {
-        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)bytes, 0x00020000);
+    const u8* base;
+    u64 kstep;
+    u32 bytes, ld, voff, piece;   // this lane's row and piece inside a group of 16 rows
+    __device__ TileSrc(const void* base_, u64 kstep_, u32 ld_, u32 bytes_, int lane)
+        : base((const u8*)base_), kstep(kstep_), bytes(bytes_), ld(ld_) {
         piece = (u32)(((lane & 3) ^ (lane >> 4)) << 4);
         voff = (u32)(lane >> 2) * (PAIRS ? 2 : 1) * ld + piece;
     }
@@ -36,16 +40,18 @@ struct TileSrc {
     __device__ static u32 source_row(u32 row) { return PAIRS ? (row & ~63u) + 2 * (row & 31) + (row >> 5 & 1) : row; }
 };
 
-// ROWS rows x 64 bytes at byte k0 of the rows into `tile`; pieces at or behind byte `kend` (a multiple of 16) become zeros
+// ROWS rows x 64 bytes of step `step` into `tile`; pieces at or behind byte `kend` (a multiple of 16) of the rows become zeros
 template <int ROWS, int WAVES, bool PAIRS>
-__device__ inline void tile_load(const TileSrc<PAIRS>& s, u32 k0, u32 kend, u8* tile, int wave) {
+__device__ inline void tile_load(const TileSrc<PAIRS>& s, u32 step, u32 kend, u8* tile, int wave) {
     static_assert(ROWS % (16 * WAVES) == 0, "every wave loads whole groups of 16 rows");
-    const u32 voff = k0 + s.piece < kend ? s.voff : 0x7ffffff0u;   // out of range: the buffer gives zeros
+    const __amdgpu_buffer_rsrc_t rsrc =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<u8*>(s.base + step * s.kstep), 0, (int)s.bytes, 0x00020000);
+    const u32 voff = step * TILE_KB + s.piece < kend ? s.voff : 0x7ffffff0u;   // out of range: the buffer gives zeros
 #pragma unroll
     for (int i = 0; i < ROWS / (16 * WAVES); i++) {
         const u32 row = (u32)(i * WAVES + wave) * 16;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(s.rsrc, (lds_void*)(tile + row * TILE_KB), 16, (int)voff,
-                                                 (int)(s.source_row(row) * s.ld + k0), 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(tile + row * TILE_KB), 16, (int)voff,
+                                                 (int)(s.source_row(row) * s.ld), 0, 0);
     }
 }
 
@@ -120,10 +126,16 @@ template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
 struct TileShape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, STAGES = STAGES_;
     static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
-    static constexpr bool PAIRS = FN == 2;   // lane c of a block of columns: 2 c, 2 c + 1
+    static constexpr bool PAIRS = FN % 2 == 0;   // lane c of blocks 2 j and 2 j + 1: columns 64 j + 2 c, 64 j + 2 c + 1
     static constexpr int STEP_BYTES = (BM + BN) * TILE_KB, LDS = STAGES * STEP_BYTES;
     static_assert(LDS <= 160 * 1024 && STAGES >= 2, "the ring fits LDS");
 };
+
+template <class S>
+__device__ inline void step_load(const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 step, u32 kend, u8* tile, int wave) {
+    tile_load<S::BM, S::WAVES, false>(p, step, kend, tile, wave);
+    tile_load<S::BN, S::WAVES, S::PAIRS>(q, step, kend, tile + S::BM * TILE_KB, wave);
+}
 
 // The order of a slice's instructions: its reads spread over its MFMAs from the first one on (left alone, the compiler moves the
 // reads back to where the next slice uses them).
@@ -137,23 +149,19 @@ __device__ inline void spread_reads() {
     }
 }
 
-// The steps at bytes [k0, kend) of the rows; kend a multiple of 16 (whole steps are read, with zeros behind kend).
+// The steps from `step` up to byte kend of the rows, kend a multiple of 16 (whole steps are read, with zeros behind kend).
 // One barrier a step: it says that the next step's tiles have landed and that everybody holds this step's last slice in
 // registers.  That slice is multiplied behind it, while the next step's first slice is on its way from LDS and the step STAGES
 // ahead (into the buffer that has just become free) on its way from memory.  Behind the last step the loads ask for nothing
 // (zeros) and the slice read is nobody's: no branch in the loop, and the count of loads in flight stays what the barrier waits for.
 template <class Kind, class S>
-__device__ inline void tile_product(Kind, const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 k0, u32 kend, u8* lds, int wave,
+__device__ inline void tile_product(Kind, const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 at, u32 kend, u8* lds, int wave,
                                     int lane, typename Kind::acc_t (&acc)[S::FM][S::FN]) {
     const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32);
     constexpr int LOADS = S::BM / (16 * S::WAVES) + S::BN / (16 * S::WAVES), KS = Kind::KS, Q = S::BM * TILE_KB;
     typedef typename Kind::template Slice<S::FM, S::FN> Slice;
-    auto load = [&](u32 k, u8* tile) {
-        tile_load<S::BM, S::WAVES>(p, k, kend, tile, wave);
-        tile_load<S::BN, S::WAVES>(q, k, kend, tile + Q, wave);
-    };
 #pragma unroll
-    for (int s = 0; s < S::STAGES; s++) load(k0 + s * TILE_KB, lds + s * S::STEP_BYTES);
+    for (int s = 0; s < S::STAGES; s++) step_load<S>(p, q, at + s, kend, lds + s * S::STEP_BYTES, wave);
     step_barrier<(S::STAGES - 1) * LOADS>();
     Slice f0, f1;
     f0.read(lds, lds + Q, wm, wn, 0, lane);
@@ -170,18 +178,18 @@ __device__ inline void tile_product(Kind, const TileSrc<false>& p, const TileSrc
         Slice& last = KS == 2 ? other : first;
         Slice& next = KS == 2 ? first : other;      // ... `first` (two slices a step) or `other` (one)
         next.read(nxt, nxt + Q, wm, wn, 0, lane);
-        load(k0 + S::STAGES * TILE_KB, cur);
+        step_load<S>(p, q, at + S::STAGES, kend, cur, wave);
         last.mul(acc);
         __builtin_amdgcn_sched_barrier(0);
         cur = nxt;
-        k0 += TILE_KB;
+        at++;
     };
+    const u32 end = (kend + TILE_KB - 1) / TILE_KB;
     if constexpr (KS == 2) {
-        while (k0 < kend) step(f0, f1);
+        while (at < end) step(f0, f1);
     } else {
-        while (k0 < kend) {
+        while (at < end) {   // a step behind the last multiplies zeros (leaving in the middle would copy the accumulators)
             step(f0, f1);
-            if (k0 >= kend) break;
             step(f1, f0);
         }
     }
