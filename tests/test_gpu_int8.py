@@ -45,7 +45,8 @@ def check_rows(I8, x, index=None):
 
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 2), (3, 5), (5, 63), (7, 64), (64, 65), (130, 127), (33, 128), (9, 1000),
-                                       (4, 1152), (3, 4096), (2, 4099), (1, 16384), (1, 40001), (70000, 3)])
+                                       (4, 1152), (3, 4096), (2, 4099), (1, 16384), (1, 40001), (70000, 3),
+                                       (2, 700001), (9, 2048), (5, 8191)])
 def test_rows(I8, dt, rows, cols):
     g = torch.Generator().manual_seed(rows * 131 + cols)
     x = torch.randn(rows, cols, generator=g) * torch.exp2(torch.randint(-12, 13, (rows, 1), generator=g).float())
@@ -74,7 +75,8 @@ def test_rows_ties_and_extremes(I8):
 
 
 @pytest.mark.parametrize("dt", list(DT))
-@pytest.mark.parametrize("cols,taps,rows", [(1, 9, 5), (3, 9, 100), (28, 9, 90), (128, 9, 84), (130, 4, 17), (16, 1, 3), (64, 30, 11)])
+@pytest.mark.parametrize("cols,taps,rows", [(1, 9, 5), (3, 9, 100), (28, 9, 90), (128, 9, 84), (130, 4, 17), (16, 1, 3), (64, 30, 11), (3000, 7, 5),
+                                             (1, 300, 4), (9000, 3, 2)])
 def test_rows_by_index(I8, dt, cols, taps, rows):
     g = torch.Generator().manual_seed(cols + taps)
     x = torch.randn(50, cols, generator=g).to(DT[dt]).cuda()
