@@ -30,6 +30,9 @@ struct Job {
     float kappa;
     double* part;
     u8 *x, *t[2], *a, *b;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
+    // short side <= 128 (see "Narrow matrices"): T in MFMA order in t, partial Gram matrices in gram
+    float* gram[2];
+    i32 nb, groups, per_group;
 };
 struct Jobs {
     Job j[MAX_JOBS];
@@ -71,10 +74,27 @@ __global__ __launch_bounds__(256) void k_ortho_norm(Jobs js, Hyper h) {
     const i64 n = (i64)J.rows * J.cols, per = (n + J.n_part - 1) / J.n_part, lo = part * per;
     const i64 hi = lo + per < n ? lo + per : n;
     double sum = 0;
-    for (i64 i = lo + threadIdx.x; i < hi; i += 256) {
-        if (h.update) J.m[i] = h.mu * J.m[i] + h.one_mu * to_f32(((const T*)J.g)[i]);
-        const double u = update_value<T>(J, h, i);
-        sum += u * u;
+    constexpr int U = 8;   // loads in flight
+    for (i64 i0 = lo + threadIdx.x; i0 < hi; i0 += 256 * U) {
+        float g[U], m[U];
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const i64 i = i0 + 256 * k < hi ? i0 + 256 * k : hi - 1;
+            g[k] = to_f32(((const T*)J.g)[i]);
+            m[k] = h.update ? J.m[i] : 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < U; k++) {
+            const i64 i = i0 + 256 * k;
+            if (i >= hi) break;
+            float u = g[k];
+            if (h.update) {
+                const float n = h.mu * m[k] + h.one_mu * u;
+                J.m[i] = n;
+                u = h.nesterov ? h.mu * n + h.one_mu * u : n;
+            }
+            sum += (double)u * u;
+        }
     }
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
@@ -252,6 +272,270 @@ using OTile128 = TileShape<128, 128, 2, 2, 4>;
 using OTile128s = TileShape<128, 64, 2, 2, 4>;   // symmetric results
 using OTile64 = TileShape<64, 64, 2, 2, 4>;
 
+// ---------------------------------------------------------------------------------------------------- Narrow matrices
+// Short side s <= 128: a launch a step.  B (s x s) fits LDS, and so does a panel of 128 values of the long index; every workgroup
+// owns some panels and
+//   1. adds the panels' partial Gram matrices that the launch before left (in order, so the sum is the same every time),
+//   2. makes B = a I + b A + c A A^T for itself,
+//   3. multiplies its panels by it, keeping T for the next launch, and adds up their part of the next Gram matrix.
+// What bounds it is latency: 5 steps of a 128 x 1152 matrix are 0.4 GFLOP, but 15 products one after the other; between launches,
+// each product would start on cold operands.
+//
+// T goes through memory in the order in which the MFMA of 3. takes it and the one before leaves it.  D = B T^T leaves lane
+// (h = lane / 32, j = lane % 32) rows i = 8 (r / 4) + 4 h + r % 4 of column j: eight registers are eight values of k for lane (h, j) of the
+// next product, if its k runs in the order that swaps bits 2 and 3 of i.  Columns of A and B in LDS are kept in that order.
+constexpr int NARROW = 128, NPANEL = 128, NTHREADS = 512, NWAVES = 8;
+constexpr int NBUF = NARROW * 512;   // a row: 128 high halves, 128 low halves
+constexpr int MAX_GROUPS = 16;       // workgroups a matrix: each adds up that many partial Gram matrices
+
+__device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
+// byte of value k of a row; pieces of 16 bytes are exchanged by row & 15, so that 16 rows read at one k use all banks
+__device__ inline int nar_off(int row, int k, int low) {
+    const int piece = low * 16 + (k >> 3);
+    return row * 512 + ((piece ^ (row & 15)) << 4) + (k & 7) * 2;
+}
+__device__ inline f16x8 nar_frag(const u8* buf, int row, int step, int h, int low) {
+    const int piece = low * 16 + 2 * step + h;
+    return *(const f16x8*)(buf + row * 512 + ((piece ^ (row & 15)) << 4));
+}
+__device__ inline void nar_put(u8* buf, int row, int k, float v) {
+    const f16 hi = (f16)v;
+    *(f16*)(buf + nar_off(row, k, 0)) = hi;
+    *(f16*)(buf + nar_off(row, k, 1)) = (f16)(v - (float)hi);
+}
+__device__ inline float nar_get(const u8* buf, int row, int k) {
+    return (float)*(const f16*)(buf + nar_off(row, k, 0)) + (float)*(const f16*)(buf + nar_off(row, k, 1));
+}
+// block b of the lower triangle of 32 x 32 blocks
+__device__ inline void lower_block(int b, int& bi, int& bj) {
+    bi = b >= 6 ? 3 : b >= 3 ? 2 : b >= 1 ? 1 : 0;
+    bj = b - bi * (bi + 1) / 2;
+}
+__device__ inline void mul3(f32x16& acc, f32x16& cross, f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl) {
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(al, bh, cross, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bh, acc, 0, 0, 0);
+    cross = __builtin_amdgcn_mfma_f32_32x32x16_f16(ah, bl, cross, 0, 0, 0);
+}
+// rows p.. of one buffer times rows q.. of another, over `steps` * 16 values
+__device__ inline void nar_block(const u8* P, int p, const u8* Q, int q, int steps, int lane, f32x16& acc) {
+    const int r = lane & 31, h = lane >> 5;
+    f32x16 cross = {};
+#pragma unroll 4
+    for (int c = 0; c < steps; c++)
+        mul3(acc, cross, nar_frag(P, p + r, c, h, 0), nar_frag(P, p + r, c, h, 1), nar_frag(Q, q + r, c, h, 0),
+             nar_frag(Q, q + r, c, h, 1));
+    acc += cross;
+}
+// a block of a symmetric matrix, both ways
+__device__ inline void nar_put_symmetric(u8* buf, int bi, int bj, int lane, const f32x16& v) {
+    const int n = bj * 32 + (lane & 31);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const int m = bi * 32 + acc_row(4 * g, lane);
+        typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float x = v[4 * g + e];
+            hi[e] = (f16)x;
+            lo[e] = (f16)(x - (float)hi[e]);
+            *(f16*)(buf + nar_off(m + e, swap23(n), 0)) = hi[e];
+            *(f16*)(buf + nar_off(m + e, swap23(n), 1)) = lo[e];
+        }
+        if (bi != bj) {   // four rows from a multiple of four on stay together
+            *(f16x4*)(buf + nar_off(n, swap23(m), 0)) = hi;
+            *(f16x4*)(buf + nar_off(n, swap23(m), 1)) = lo;
+        }
+    }
+}
+__device__ inline int nar_blocks(const Job& J) { return J.nb * (J.nb + 1) / 2; }
+// this wave's blocks (wave, wave + 8) of the panel's Gram matrix; the panel is in buf as [short index][long index]
+__device__ inline void nar_gram(const Job& J, const u8* buf, int wave, int lane, f32x16 (&acc)[2]) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int b = wave + NWAVES * x;
+        if (b >= nar_blocks(J)) continue;
+        int bi, bj;
+        lower_block(b, bi, bj);
+        nar_block(buf, bi * 32, buf, bj * 32, NPANEL / 16, lane, acc[x]);
+    }
+}
+__device__ inline void nar_gram_store(const Job& J, float* gram, int group, int wave, int lane, const f32x16 (&acc)[2]) {
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int b = wave + NWAVES * x;
+        if (b >= nar_blocks(J)) continue;
+        float* d = gram + ((i64)(group * nar_blocks(J) + b) * 64 + lane) * 16;
+#pragma unroll
+        for (int g = 0; g < 4; g++) *(f32x4*)(d + 4 * g) = f32x4{acc[x][4 * g], acc[x][4 * g + 1], acc[x][4 * g + 2], acc[x][4 * g + 3]};
+    }
+}
+// T of panel p, long-index block jb (32 values), k step c: 64 lanes x 16 bytes
+__device__ inline u8* nar_t(u8* t, int p, int jb, int c, int low) { return t + ((((i64)p * 4 + jb) * 8 + c) * 2 + low) * 1024; }
+
+template <class T>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_init(Jobs js, Hyper h) {
+    extern __shared__ __attribute__((aligned(128))) u8 lds[];
+    __shared__ double red[NWAVES];
+    const int ji = find_job(js, blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job& J = js.j[ji];
+    const int group = blockIdx.x - js.first[ji], panels = (J.l + NPANEL - 1) / NPANEL, height = J.nb * 32;
+    const bool flip = J.rows > J.cols;
+    double sum = 0;
+    for (int i = tid; i < J.n_part; i += NTHREADS) sum += J.part[i];
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int i = 0; i < NWAVES; i++) sum += red[i];
+    const float scale = (float)(16384.0 / (sqrt(sum) + h.eps));
+    f32x16 acc[2] = {};
+    for (int p = group * J.per_group; p < panels && p < (group + 1) * J.per_group; p++) {
+        const int j0 = p * NPANEL;
+#pragma unroll 8
+        for (int e = tid; e < height * NPANEL; e += NTHREADS) {   // consecutive threads along the matrix's rows in memory
+            const int i = flip ? e % height : e / NPANEL, j = flip ? e / height : e % NPANEL;
+            float v = 0;
+            if (i < J.s && j0 + j < J.l)
+                v = update_value<T>(J, h, flip ? (i64)(j0 + j) * J.cols + i : (i64)i * J.cols + j0 + j) * scale;
+            nar_put(lds, i, j, v);
+        }
+        __syncthreads();
+        const int jb = wave & 3, hh = lane >> 5, j = jb * 32 + (lane & 31);
+        for (int c = (wave >> 2) * 4; c < (wave >> 2) * 4 + 4 && c < 2 * J.nb; c++)
+            for (int low = 0; low < 2; low++) {
+                f16x8 f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[e] = *(const f16*)(lds + nar_off(16 * c + swap23(8 * hh + e), j, low));
+                *(f16x8*)(nar_t(J.t[0], p, jb, c, low) + lane * 16) = f;
+            }
+        nar_gram(J, lds, wave, lane, acc);
+        __syncthreads();
+    }
+    nar_gram_store(J, J.gram[0], group, wave, lane, acc);
+}
+
+template <class T, bool LASTSTEP>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int cur) {
+    extern __shared__ __attribute__((aligned(128))) u8 lds[];
+    u8 *const bufA = lds, *const bufB = lds + NBUF;   // A, then the new panel; B
+    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Job& J = js.j[ji];
+    const int group = blockIdx.x - js.first[ji], panels = (J.l + NPANEL - 1) / NPANEL, blocks = nar_blocks(J), steps = 2 * J.nb;
+    const int first = group * J.per_group, end = first + J.per_group < panels ? first + J.per_group : panels;
+    const bool flip = J.rows > J.cols;
+    const int jb = wave & 3, ib = (wave >> 2) * 2;   // this wave: 32 of the panel's long index, short-index blocks ib, ib + 1
+    f16x8 t[8][2];
+    auto fetch = [&](int p) {
+#pragma unroll
+        for (int c = 0; c < 8; c++)
+            if (c < steps)
+#pragma unroll
+                for (int low = 0; low < 2; low++) t[c][low] = *(const f16x8*)(nar_t(J.t[cur], p, jb, c, low) + lane * 16);
+    };
+    if (first < end) fetch(first);
+    // 1. A = sum of the groups' parts
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int b = wave + NWAVES * x;
+        if (b >= blocks) continue;
+        f32x16 v = {};
+        for (int g = 0; g < J.groups; g++) {
+            const f32x4* d = (const f32x4*)(J.gram[cur] + ((i64)(g * blocks + b) * 64 + lane) * 16);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const f32x4 y = d[k];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[4 * k + e] += y[e];
+            }
+        }
+        int bi, bj;
+        lower_block(b, bi, bj);
+        nar_put_symmetric(bufA, bi, bj, lane, v * 0x1p-16f);
+    }
+    __syncthreads();
+    // 2. B
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+        const int b = wave + NWAVES * x;
+        if (b >= blocks) continue;
+        int bi, bj;
+        lower_block(b, bi, bj);
+        f32x16 acc = {};
+        nar_block(bufA, bi * 32, bufA, bj * 32, steps, lane, acc);
+        const int n = bj * 32 + (lane & 31);
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const int m = bi * 32 + acc_row(r, lane);
+            const float A = nar_get(bufA, m, swap23(n)) * 0x1p-12f;
+            acc[r] = (h.c * (acc[r] * 0x1p-24f) + h.b * A + (m == n ? h.a : 0.0f)) * 0x1p11f;
+        }
+        nar_put_symmetric(bufB, bi, bj, lane, acc);
+    }
+    __syncthreads();
+    // 3. the panels
+    f32x16 gram[2] = {};
+    for (int p = first; p < end; p++) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+            if (ib + x >= J.nb) continue;
+            const int i0 = (ib + x) * 32, hh = lane >> 5;
+            f32x16 acc = {}, cross = {};
+            const bool across = LASTSTEP && flip;   // the output's rows are the long index: lanes along the short one
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                if (c >= steps) continue;
+                const f16x8 bh = nar_frag(bufB, i0 + (lane & 31), c, hh, 0), bl = nar_frag(bufB, i0 + (lane & 31), c, hh, 1);
+                if (across) mul3(acc, cross, t[c][0], t[c][1], bh, bl);
+                else mul3(acc, cross, bh, bl, t[c][0], t[c][1]);
+            }
+            acc += cross;
+            if (!LASTSTEP) {
+                acc *= 0x1p-11f;
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    f16x8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float v = acc[8 * half + e];
+                        hi[e] = (f16)v;
+                        lo[e] = (f16)(v - (float)hi[e]);
+                        const int i = i0 + acc_row(8 * half + e, lane), j = jb * 32 + (lane & 31);
+                        *(f16*)(bufA + nar_off(i, j, 0)) = hi[e];
+                        *(f16*)(bufA + nar_off(i, j, 1)) = lo[e];
+                    }
+                    const int c = 2 * (ib + x) + half;
+                    *(f16x8*)(nar_t(J.t[cur ^ 1], p, jb, c, 0) + lane * 16) = hi;
+                    *(f16x8*)(nar_t(J.t[cur ^ 1], p, jb, c, 1) + lane * 16) = lo;
+                }
+            } else {
+                const int col = (across ? i0 : p * NPANEL + jb * 32) + (lane & 31), row0 = across ? p * NPANEL + jb * 32 : i0;
+                float old[16];
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int row = row0 + acc_row(r, lane);
+                    old[r] = h.update && row < J.rows && col < J.cols ? to_f32(((const T*)J.w)[(i64)row * J.cols + col]) : 0.0f;
+                }
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int row = row0 + acc_row(r, lane);
+                    if (row >= J.rows || col >= J.cols) continue;
+                    float o = acc[r] * 0x1p-25f;
+                    if (h.update) o = old[r] * h.decay - o * (h.lr * J.kappa);
+                    ((T*)J.w)[(i64)row * J.cols + col] = from_f32<T>(o);
+                }
+            }
+        }
+        if (p + 1 < end) fetch(p + 1);
+        if (!LASTSTEP) {
+            __syncthreads();
+            nar_gram(J, bufA, wave, lane, gram);
+            __syncthreads();
+        }
+    }
+    if (!LASTSTEP) nar_gram_store(J, J.gram[cur ^ 1], group, wave, lane, gram);
+}
+
 // ---------------------------------------------------------------------------------------------------- host side
 static i64 pad(i64 n) { return (n + OT - 1) / OT * OT; }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -275,6 +559,20 @@ static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
         return (u8*)r;
     };
     J.part = (double*)take(J.n_part * sizeof(double));
+    J.nb = (J.s + 31) / 32;
+    if (J.s <= NARROW) {
+        const int panels = (J.l + NPANEL - 1) / NPANEL;
+        J.per_group = (panels + MAX_GROUPS - 1) / MAX_GROUPS;
+        J.groups = (panels + J.per_group - 1) / J.per_group;
+        for (int i = 0; i < 2; i++) {
+            J.t[i] = take((size_t)panels * NPANEL * NARROW * 4);
+            J.gram[i] = (float*)take((size_t)J.groups * (J.nb * (J.nb + 1) / 2) * 4096);
+        }
+        J.x = J.a = J.b = nullptr;
+        return off;
+    }
+    J.gram[0] = J.gram[1] = nullptr;
+    J.groups = J.per_group = 0;
     J.x = take((size_t)J.sp * J.lp * 4);
     J.t[0] = take((size_t)J.sp * J.lp * 4);
     J.t[1] = take((size_t)J.sp * J.lp * 4);
@@ -336,7 +634,29 @@ static void product(Jobs& js, const Hyper& h, int cur, hipStream_t st) {
     k_ortho_product<MODE, OTile64, T><<<dim3((u32)n), dim3(OTile64::THREADS), Staged<OTile64>::LDS, st>>>(js, h, cur);
 }
 
-static int run_jobs(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
+static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
+    each_first(js, [](const Job& J) { return J.n_part; });
+    AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
+    each_first(js, [](const Job& J) { return J.groups; });
+    const dim3 grid(js.first[js.n]), block(NTHREADS);
+    AZ_DISPATCH_DTYPE(dtype, k_narrow_init<T><<<grid, block, NBUF, st>>>(js, h));
+    for (int it = 0; it + 1 < steps; it++) k_narrow_step<float, false><<<grid, block, 2 * NBUF, st>>>(js, h, it & 1);
+    AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true><<<grid, block, 2 * NBUF, st>>>(js, h, (steps - 1) & 1));
+    return launch_status("az_orthogonalize");
+}
+
+static int run_jobs(Jobs& all, const Hyper& h, int steps, int dtype, hipStream_t st) {
+    Jobs js;
+    js.n = 0;
+    for (int i = 0; i < all.n; i++)
+        if (all.j[i].s <= NARROW) js.j[js.n++] = all.j[i];
+    if (js.n) {
+        const int rc = run_narrow(js, h, steps, dtype, st);
+        if (rc != AZ_OK || js.n == all.n) return rc;
+    }
+    js.n = 0;
+    for (int i = 0; i < all.n; i++)
+        if (all.j[i].s > NARROW) js.j[js.n++] = all.j[i];
     each_first(js, [](const Job& J) { return J.n_part; });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
