@@ -29,9 +29,10 @@ struct Job {
     i32 rows, cols, s, l, sp, lp, n_part;
     float kappa;
     double* part;
-    u8 *x, *t[2], *a, *b;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
+    u8 *x, *t0, *t1, *a, *b;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
     // short side <= 128 (see "Narrow matrices"): T in MFMA order in t, partial Gram matrices in gram
-    float* gram[2];
+    float* gram;
+    u8* image;
     i32 nb, groups, per_group;
 };
 struct Jobs {
@@ -50,26 +51,52 @@ __device__ inline int find_job(const Jobs& js, int block) {
     while (j + 1 < js.n && block >= js.first[j + 1]) j++;
     return j;
 }
-template <class T>
-__device__ inline float update_value(const Job& J, const Hyper& h, i64 i) {   // after k_ortho_norm has updated m
-    const float g = to_f32(((const T*)J.g)[i]);
-    if (!h.update) return g;
-    const float m = J.m[i];
-    return h.nesterov ? h.mu * m + h.one_mu * g : m;
-}
-__device__ inline void split_store(u8* p, float v) {   // p: the high half's place
-    const f16 hi = (f16)v;
-    *(f16*)p = hi;
-    *(f16*)(p + 32) = (f16)(v - (float)hi);
+// Loads above stay above (left alone, the compiler moves each one to its use to save registers, and every one waits for memory).
+__device__ inline void loads_first() { __builtin_amdgcn_sched_barrier(0); }
+
+// what is orthogonalised, after k_ortho_norm has updated m: N values a thread, at `at` (where `in`; else zeros)
+template <class T, int N>
+__device__ inline void update_values(const Job& J, const Hyper& h, const i32 (&at)[N], const bool (&in)[N], float (&v)[N]) {
+    T g[N];
+    float m[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) g[k] = ((const T*)J.g)[in[k] ? at[k] : 0];
+    if (h.update)
+#pragma unroll
+        for (int k = 0; k < N; k++) m[k] = J.m[in[k] ? at[k] : 0];
+    loads_first();
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        v[k] = to_f32(g[k]);
+        if (h.update) v[k] = h.nesterov ? h.mu * m[k] + h.one_mu * v[k] : m[k];
+        if (!in[k]) v[k] = 0;
+    }
 }
 __device__ inline i64 split_off(i64 row, i64 rows, i64 k) { return ((k >> 4) * rows + row) * TILE_KB + (k & 15) * 2; }
+
+// eight values of a row from a multiple of eight on: their halves, 16 bytes each
+__device__ inline void split_store8(u8* p, const float (&v)[8]) {
+    f16x8 hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        hi[e] = (f16)v[e];
+        lo[e] = (f16)(v[e] - (float)hi[e]);
+    }
+    *(f16x8*)p = hi;
+    *(f16x8*)(p + 32) = lo;
+}
+__device__ inline void split_load8(const u8* p, float (&v)[8]) {
+    const f16x8 hi = *(const f16x8*)p, lo = *(const f16x8*)(p + 32);
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)hi[e] + (float)lo[e];
+}
 
 // momentum (in place) and partial sums of squares of the update, in float64: the squares of float32 values can leave float32
 template <class T>
 __global__ __launch_bounds__(256) void k_ortho_norm(Jobs js, Hyper h) {
     __shared__ double red[4];
     const int ji = find_job(js, blockIdx.x);
-    const Job& J = js.j[ji];
+    const Job J = js.j[ji];
     const int part = blockIdx.x - js.first[ji];
     const i64 n = (i64)J.rows * J.cols, per = (n + J.n_part - 1) / J.n_part, lo = part * per;
     const i64 hi = lo + per < n ? lo + per : n;
@@ -83,6 +110,7 @@ __global__ __launch_bounds__(256) void k_ortho_norm(Jobs js, Hyper h) {
             g[k] = to_f32(((const T*)J.g)[i]);
             m[k] = h.update ? J.m[i] : 0.0f;
         }
+        loads_first();
 #pragma unroll
         for (int k = 0; k < U; k++) {
             const i64 i = i0 + 256 * k;
@@ -108,7 +136,7 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     __shared__ float tile[OT][OT + 1];   // [short index][long index]
     __shared__ double red[4];
     const int ji = find_job(js, blockIdx.x), tid = threadIdx.x;
-    const Job& J = js.j[ji];
+    const Job J = js.j[ji];
     const int nl = J.lp / OT, tl = blockIdx.x - js.first[ji], i0 = tl / nl * OT, j0 = tl % nl * OT;
     double sum = 0;
     for (int i = tid; i < J.n_part; i += 256) sum += J.part[i];
@@ -117,37 +145,35 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     __syncthreads();
     const float scale = (float)(16384.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + h.eps));
     const bool flip = J.rows > J.cols;
-    for (int e = tid; e < OT * OT; e += 256) {
-        const int hi_ = e / OT, lo_ = e % OT;           // lo_ runs along the matrix's rows in memory
-        const int i = flip ? lo_ : hi_, j = flip ? hi_ : lo_;
-        float v = 0;
-        if (i0 + i < J.s && j0 + j < J.l)
-            v = update_value<T>(J, h, flip ? (i64)(j0 + j) * J.cols + i0 + i : (i64)(i0 + i) * J.cols + j0 + j) * scale;
-        tile[i][j] = v;
+    constexpr int U = 16;   // values a thread, all on their way at once
+    float v[U];
+    i32 at[U];   // rows * cols <= 2^30
+    bool in[U];
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+        const int e = tid + 256 * k, slow = e / OT, fast = e % OT;   // fast runs along the matrix's rows in memory
+        const int i = flip ? fast : slow, j = flip ? slow : fast;
+        in[k] = i0 + i < J.s && j0 + j < J.l;
+        at[k] = flip ? (j0 + j) * J.cols + i0 + i : (i0 + i) * J.cols + j0 + j;
+    }
+    update_values<T>(J, h, at, in, v);
+#pragma unroll
+    for (int k = 0; k < U; k++) {
+        const int e = tid + 256 * k, slow = e / OT, fast = e % OT;
+        tile[flip ? fast : slow][flip ? slow : fast] = v[k] * scale;
     }
     __syncthreads();
-    for (int e = tid; e < OT * OT; e += 256) {
-        const int r = e / OT, c = e % OT;
-        split_store(J.x + split_off(i0 + r, J.sp, j0 + c), tile[r][c]);
-        split_store(J.t[0] + split_off(j0 + r, J.lp, i0 + c), tile[c][r]);
-    }
-}
-
-// eight values of a row from a multiple of eight on: their halves, 16 bytes each
-__device__ inline void split_store8(u8* p, const float (&v)[8]) {
-    f16x8 hi, lo;
+    for (int u = tid; u < OT * OT / 8; u += 256) {   // pairs of lanes: 16 values of a row, 64 bytes
+        const int r = u / 2 % OT, c = (u % 2 + u / (2 * OT) * 2) * 8;
+        float a[8], b[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        hi[e] = (f16)v[e];
-        lo[e] = (f16)(v[e] - (float)hi[e]);
+        for (int e = 0; e < 8; e++) {
+            a[e] = tile[r][c + e];
+            b[e] = tile[c + e][r];
+        }
+        split_store8(J.x + split_off(i0 + r, J.sp, j0 + c), a);
+        split_store8(J.t0 + split_off(j0 + r, J.lp, i0 + c), b);
     }
-    *(f16x8*)p = hi;
-    *(f16x8*)(p + 32) = lo;
-}
-__device__ inline void split_load8(const u8* p, float (&v)[8]) {
-    const f16x8 hi = *(const f16x8*)p, lo = *(const f16x8*)(p + 32);
-#pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = (float)hi[e] + (float)lo[e];
 }
 
 enum { GRAM = 0, POLY = 1, STEP = 2, LAST = 3 };
@@ -179,16 +205,17 @@ template <int MODE, class S, class T>
 __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     const int ji = find_job(js, blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Job& J = js.j[ji];
+    const Job J = js.j[ji];
     const bool flip = J.rows > J.cols;
     constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    u8 *const t_cur = cur ? J.t1 : J.t0, *const t_next = cur ? J.t0 : J.t1;
     const u8 *P, *Q;
     int kp, rows, cols;
     product_dims(MODE, J, rows, cols);
     if (MODE == GRAM) { P = Q = J.x; kp = J.lp; }
     else if (MODE == POLY) { P = Q = J.a; kp = J.sp; }
-    else if (MODE == STEP || flip) { P = J.t[cur]; Q = J.b; kp = J.sp; }
-    else { P = J.b; Q = J.t[cur]; kp = J.sp; }
+    else if (MODE == STEP || flip) { P = t_cur; Q = J.b; kp = J.sp; }
+    else { P = J.b; Q = t_cur; kp = J.sp; }
     u32 tm, tn;
     const int block = blockIdx.x - js.first[ji];
     if (SYM) {
@@ -223,7 +250,7 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
             }
     __syncthreads();
     if (MODE != LAST) {   // mrows and ncols are multiples of 64 here
-        u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : J.t[cur ^ 1];
+        u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : t_next;
         // pairs of lanes store 16 values of a row, 64 bytes; the next pair those of the next row, right behind them
         for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
             const int r = u / 2 % S::BM, c = (u % 2 + u / (2 * S::BM) * 2) * 8, m = m0 + r, n = n0 + c;
@@ -273,9 +300,10 @@ using OTile128s = TileShape<128, 64, 2, 2, 4>;   // symmetric results
 using OTile64 = TileShape<64, 64, 2, 2, 4>;
 
 // ---------------------------------------------------------------------------------------------------- Narrow matrices
-// Short side s <= 128: a launch a step.  B (s x s) fits LDS, and so does a panel of 128 values of the long index; every workgroup
-// owns some panels and
-//   1. adds the panels' partial Gram matrices that the launch before left (in order, so the sum is the same every time),
+// Short side s <= 128: two launches a step.  B (s x s) fits LDS, and so does a panel of 128 values of the long index.  The first
+// launch adds up the panels' parts of A = X X^T (in order, so the sum is the same every time); in the second every workgroup owns
+// some panels and
+//   1. takes A into LDS,
 //   2. makes B = a I + b A + c A A^T for itself,
 //   3. multiplies its panels by it, keeping T for the next launch, and adds up their part of the next Gram matrix.
 // What bounds it is latency: 5 steps of a 128 x 1152 matrix are 0.4 GFLOP, but 15 products one after the other; between launches,
@@ -284,8 +312,9 @@ using OTile64 = TileShape<64, 64, 2, 2, 4>;
 // T goes through memory in the order in which the MFMA of 3. takes it and the one before leaves it.  D = B T^T leaves lane
 // (h = lane / 32, j = lane % 32) rows i = 8 (r / 4) + 4 h + r % 4 of column j: eight registers are eight values of k for lane (h, j) of the
 // next product, if its k runs in the order that swaps bits 2 and 3 of i.  Columns of A and B in LDS are kept in that order.
-constexpr int NARROW = 128, NPANEL = 128, NTHREADS = 512, NWAVES = 8;
+constexpr int NARROW = 128, NPANEL = 128, NTHREADS = 1024, NWAVES = 16;
 constexpr int NBUF = NARROW * 512;   // a row: 128 high halves, 128 low halves
+constexpr int NSTEP_LDS = 2 * NBUF + 32 * 1024;
 constexpr int MAX_GROUPS = 16;       // workgroups a matrix: each adds up that many partial Gram matrices
 
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
@@ -303,9 +332,6 @@ __device__ inline void nar_put(u8* buf, int row, int k, float v) {
     *(f16*)(buf + nar_off(row, k, 0)) = hi;
     *(f16*)(buf + nar_off(row, k, 1)) = (f16)(v - (float)hi);
 }
-__device__ inline float nar_get(const u8* buf, int row, int k) {
-    return (float)*(const f16*)(buf + nar_off(row, k, 0)) + (float)*(const f16*)(buf + nar_off(row, k, 1));
-}
 // block b of the lower triangle of 32 x 32 blocks
 __device__ inline void lower_block(int b, int& bi, int& bj) {
     bi = b >= 6 ? 3 : b >= 3 ? 2 : b >= 1 ? 1 : 0;
@@ -320,55 +346,42 @@ __device__ inline void mul3(f32x16& acc, f32x16& cross, f16x8 ah, f16x8 al, f16x
 __device__ inline void nar_block(const u8* P, int p, const u8* Q, int q, int steps, int lane, f32x16& acc) {
     const int r = lane & 31, h = lane >> 5;
     f32x16 cross = {};
-#pragma unroll 4
+#pragma unroll 1
     for (int c = 0; c < steps; c++)
         mul3(acc, cross, nar_frag(P, p + r, c, h, 0), nar_frag(P, p + r, c, h, 1), nar_frag(Q, q + r, c, h, 0),
              nar_frag(Q, q + r, c, h, 1));
     acc += cross;
 }
-// a block of a symmetric matrix, both ways
-__device__ inline void nar_put_symmetric(u8* buf, int bi, int bj, int lane, const f32x16& v) {
-    const int n = bj * 32 + (lane & 31);
+typedef f16 f16x4 __attribute__((ext_vector_type(4)));
+// rows m..m + 3 (a multiple of four on) of column n of a symmetric matrix, as row n, columns m..m + 3: they stay together there
+__device__ inline void nar_put4(u8* buf, int m, int n, const float (&v)[4]) {
+    f16x4 hi, lo;
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        const int m = bi * 32 + acc_row(4 * g, lane);
-        typedef f16 f16x4 __attribute__((ext_vector_type(4)));
-        f16x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float x = v[4 * g + e];
-            hi[e] = (f16)x;
-            lo[e] = (f16)(x - (float)hi[e]);
-            *(f16*)(buf + nar_off(m + e, swap23(n), 0)) = hi[e];
-            *(f16*)(buf + nar_off(m + e, swap23(n), 1)) = lo[e];
-        }
-        if (bi != bj) {   // four rows from a multiple of four on stay together
-            *(f16x4*)(buf + nar_off(n, swap23(m), 0)) = hi;
-            *(f16x4*)(buf + nar_off(n, swap23(m), 1)) = lo;
-        }
+    for (int e = 0; e < 4; e++) {
+        hi[e] = (f16)v[e];
+        lo[e] = (f16)(v[e] - (float)hi[e]);
     }
+    *(f16x4*)(buf + nar_off(n, swap23(m), 0)) = hi;
+    *(f16x4*)(buf + nar_off(n, swap23(m), 1)) = lo;
+}
+__device__ inline void nar_get4(const u8* buf, int m, int n, float (&v)[4]) {
+    const f16x4 hi = *(const f16x4*)(buf + nar_off(n, swap23(m), 0)), lo = *(const f16x4*)(buf + nar_off(n, swap23(m), 1));
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = (float)hi[e] + (float)lo[e];
 }
 __device__ inline int nar_blocks(const Job& J) { return J.nb * (J.nb + 1) / 2; }
-// this wave's blocks (wave, wave + 8) of the panel's Gram matrix; the panel is in buf as [short index][long index]
-__device__ inline void nar_gram(const Job& J, const u8* buf, int wave, int lane, f32x16 (&acc)[2]) {
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int b = wave + NWAVES * x;
-        if (b >= nar_blocks(J)) continue;
-        int bi, bj;
-        lower_block(b, bi, bj);
-        nar_block(buf, bi * 32, buf, bj * 32, NPANEL / 16, lane, acc[x]);
-    }
+// this wave's block of the panel's Gram matrix (10 at most); the panel is in buf as [short index][long index]
+__device__ inline void nar_gram(const Job& J, const u8* buf, int wave, int lane, f32x16& acc) {
+    if (wave >= nar_blocks(J)) return;
+    int bi, bj;
+    lower_block(wave, bi, bj);
+    nar_block(buf, bi * 32, buf, bj * 32, NPANEL / 16, lane, acc);
 }
-__device__ inline void nar_gram_store(const Job& J, float* gram, int group, int wave, int lane, const f32x16 (&acc)[2]) {
+__device__ inline void nar_gram_store(const Job& J, int group, int wave, int lane, const f32x16& acc) {
+    if (wave >= nar_blocks(J)) return;
+    float* d = J.gram + ((i64)(group * nar_blocks(J) + wave) * 64 + lane) * 16;
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int b = wave + NWAVES * x;
-        if (b >= nar_blocks(J)) continue;
-        float* d = gram + ((i64)(group * nar_blocks(J) + b) * 64 + lane) * 16;
-#pragma unroll
-        for (int g = 0; g < 4; g++) *(f32x4*)(d + 4 * g) = f32x4{acc[x][4 * g], acc[x][4 * g + 1], acc[x][4 * g + 2], acc[x][4 * g + 3]};
-    }
+    for (int g = 0; g < 4; g++) *(f32x4*)(d + 4 * g) = f32x4{acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
 }
 // T of panel p, long-index block jb (32 values), k step c: 64 lanes x 16 bytes
 __device__ inline u8* nar_t(u8* t, int p, int jb, int c, int low) { return t + ((((i64)p * 4 + jb) * 8 + c) * 2 + low) * 1024; }
@@ -377,9 +390,11 @@ template <class T>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_init(Jobs js, Hyper h) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     __shared__ double red[NWAVES];
-    const int ji = find_job(js, blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Job& J = js.j[ji];
-    const int group = blockIdx.x - js.first[ji], panels = (J.l + NPANEL - 1) / NPANEL, height = J.nb * 32;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Job J = js.j[blockIdx.y];
+    const int group = blockIdx.x;
+    if (group >= J.groups) return;
+    const int panels = (J.l + NPANEL - 1) / NPANEL, height = J.nb * 32;
     const bool flip = J.rows > J.cols;
     double sum = 0;
     for (int i = tid; i < J.n_part; i += NTHREADS) sum += J.part[i];
@@ -389,105 +404,152 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_init(Jobs js, Hyper h) {
     sum = 0;
     for (int i = 0; i < NWAVES; i++) sum += red[i];
     const float scale = (float)(16384.0 / (sqrt(sum) + h.eps));
-    f32x16 acc[2] = {};
+    f32x16 acc = {};
     for (int p = group * J.per_group; p < panels && p < (group + 1) * J.per_group; p++) {
         const int j0 = p * NPANEL;
-#pragma unroll 8
-        for (int e = tid; e < height * NPANEL; e += NTHREADS) {   // consecutive threads along the matrix's rows in memory
-            const int i = flip ? e % height : e / NPANEL, j = flip ? e / height : e % NPANEL;
-            float v = 0;
-            if (i < J.s && j0 + j < J.l)
-                v = update_value<T>(J, h, flip ? (i64)(j0 + j) * J.cols + i : (i64)i * J.cols + j0 + j) * scale;
-            nar_put(lds, i, j, v);
+        // consecutive threads along the matrix's rows in memory; 8 values a thread on their way at once
+        constexpr int U = 8;
+        static_assert(NARROW * NPANEL % (NTHREADS * U) == 0, "whole rounds");
+#pragma unroll 1
+        for (int e0 = tid; e0 < NARROW * NPANEL; e0 += NTHREADS * U) {
+            float v[U];
+            i32 at[U];   // rows * cols <= 2^30
+            bool in[U];
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int e = e0 + NTHREADS * k, i = flip ? e % NARROW : e / NPANEL, j = flip ? e / NARROW : e % NPANEL;
+                in[k] = i < J.s && j0 + j < J.l;
+                at[k] = flip ? (j0 + j) * J.cols + i : i * J.cols + j0 + j;
+            }
+            update_values<T>(J, h, at, in, v);
+#pragma unroll
+            for (int k = 0; k < U; k++) {
+                const int e = e0 + NTHREADS * k, i = flip ? e % NARROW : e / NPANEL, j = flip ? e / NARROW : e % NPANEL;
+                if (i < height) nar_put(lds, i, j, v[k] * scale);
+            }
         }
         __syncthreads();
         const int jb = wave & 3, hh = lane >> 5, j = jb * 32 + (lane & 31);
-        for (int c = (wave >> 2) * 4; c < (wave >> 2) * 4 + 4 && c < 2 * J.nb; c++)
+        for (int c = (wave >> 2) * 2; c < (wave >> 2) * 2 + 2 && c < 2 * J.nb; c++)
             for (int low = 0; low < 2; low++) {
                 f16x8 f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[e] = *(const f16*)(lds + nar_off(16 * c + swap23(8 * hh + e), j, low));
-                *(f16x8*)(nar_t(J.t[0], p, jb, c, low) + lane * 16) = f;
+                *(f16x8*)(nar_t(J.t0, p, jb, c, low) + lane * 16) = f;
             }
         nar_gram(J, lds, wave, lane, acc);
         __syncthreads();
     }
-    nar_gram_store(J, J.gram[0], group, wave, lane, acc);
+    nar_gram_store(J, group, wave, lane, acc);
+}
+
+// A = sum of the groups' parts (in order), as the image that k_narrow_step takes into LDS: a block a workgroup.  A launch of its
+// own: every workgroup of k_narrow_step adding up 40 KB from each of 9 others took 11 of its 24 us.
+__global__ __launch_bounds__(256) void k_narrow_sum(Jobs js) {
+    const Job J = js.j[blockIdx.y];
+    const int blocks = nar_blocks(J), b = blockIdx.x, lane = threadIdx.x & 63, g4 = threadIdx.x >> 6;
+    if (b >= blocks) return;
+    const float* d = J.gram + ((i64)b * 64 + lane) * 16 + 4 * g4;
+    f32x4 y[MAX_GROUPS], sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int g = 0; g < MAX_GROUPS; g++) y[g] = *(const f32x4*)(d + (i64)(g < J.groups ? g : 0) * blocks * 1024);
+    loads_first();
+#pragma unroll
+    for (int g = 0; g < MAX_GROUPS; g++)
+        if (g < J.groups) sum += y[g];
+    int bi, bj;
+    lower_block(b, bi, bj);
+    const int m = bi * 32 + acc_row(4 * g4, lane), n = bj * 32 + (lane & 31);
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = sum[e] * 0x1p-16f;
+    nar_put4(J.image, m, n, v);
+    if (bi != bj)
+#pragma unroll
+        for (int e = 0; e < 4; e++) nar_put(J.image, m + e, swap23(n), v[e]);
 }
 
 template <class T, bool LASTSTEP>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int cur) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     u8 *const bufA = lds, *const bufB = lds + NBUF;   // A, then the new panel; B
-    const int ji = find_job(js, blockIdx.x), lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Job& J = js.j[ji];
-    const int group = blockIdx.x - js.first[ji], panels = (J.l + NPANEL - 1) / NPANEL, blocks = nar_blocks(J), steps = 2 * J.nb;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Job J = js.j[blockIdx.y];   // no search: what a launch waits for first is its arguments, one line after the other
+    if ((int)blockIdx.x >= J.groups) return;
+    u8 *const t_cur = cur ? J.t1 : J.t0, *const t_next = cur ? J.t0 : J.t1;
+    const int group = blockIdx.x, panels = (J.l + NPANEL - 1) / NPANEL, steps = 2 * J.nb;
     const int first = group * J.per_group, end = first + J.per_group < panels ? first + J.per_group : panels;
     const bool flip = J.rows > J.cols;
-    const int jb = wave & 3, ib = (wave >> 2) * 2;   // this wave: 32 of the panel's long index, short-index blocks ib, ib + 1
-    f16x8 t[8][2];
+    const int jb = wave & 3, ib = wave >> 2;   // this wave: 32 of the panel's long index, a block of the short one
+    // 1. A
+    {
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(J.image, 0, J.nb * 32 * 512, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NBUF / 1024 / NWAVES; i++) {   // rows behind nb blocks: zeros
+            const int at = (i * NWAVES + wave) * 1024;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(bufA + at), 16, lane * 16, at, 0, 0);
+        }
+    }
+    // T of a panel: k steps 0..3 in registers, 4..7 through LDS (64 registers more than a wave has)
+    u8* const bufT = lds + 2 * NBUF;
+    f16x8 t[4][2];
     auto fetch = [&](int p) {
 #pragma unroll
-        for (int c = 0; c < 8; c++)
-            if (c < steps)
+        for (int c = 0; c < 4; c++)
 #pragma unroll
-                for (int low = 0; low < 2; low++) t[c][low] = *(const f16x8*)(nar_t(J.t[cur], p, jb, c, low) + lane * 16);
+            for (int low = 0; low < 2; low++) t[c][low] = *(const f16x8*)(nar_t(t_cur, p, jb, c < steps ? c : 0, low) + lane * 16);
     };
-    if (first < end) fetch(first);
-    // 1. A = sum of the groups' parts
+    auto fetch_high = [&](int p) {   // waves of one jb: a k step each
+        if (4 + ib >= steps) return;
+        const u8* src = nar_t(t_cur, p, jb, 4 + ib, 0);
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<u8*>(src), 0, 2048, 0x00020000);
 #pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int b = wave + NWAVES * x;
-        if (b >= blocks) continue;
-        f32x16 v = {};
-        for (int g = 0; g < J.groups; g++) {
-            const f32x4* d = (const f32x4*)(J.gram[cur] + ((i64)(g * blocks + b) * 64 + lane) * 16);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const f32x4 y = d[k];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[4 * k + e] += y[e];
-            }
-        }
-        int bi, bj;
-        lower_block(b, bi, bj);
-        nar_put_symmetric(bufA, bi, bj, lane, v * 0x1p-16f);
-    }
+        for (int low = 0; low < 2; low++)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(bufT + ((jb * 4 + ib) * 2 + low) * 1024), 16, lane * 16, low * 1024, 0, 0);
+    };
+    fetch_high(first);
+    fetch(first);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    // 2. B
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-        const int b = wave + NWAVES * x;
-        if (b >= blocks) continue;
-        int bi, bj;
-        lower_block(b, bi, bj);
+    // 2. B, every block of it
+    if (wave < J.nb * J.nb) {
+        const int bi = wave / J.nb, bj = wave - bi * J.nb, n = bj * 32 + (lane & 31);
         f32x16 acc = {};
         nar_block(bufA, bi * 32, bufA, bj * 32, steps, lane, acc);
-        const int n = bj * 32 + (lane & 31);
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const int m = bi * 32 + acc_row(r, lane);
-            const float A = nar_get(bufA, m, swap23(n)) * 0x1p-12f;
-            acc[r] = (h.c * (acc[r] * 0x1p-24f) + h.b * A + (m == n ? h.a : 0.0f)) * 0x1p11f;
+        for (int g = 0; g < 4; g++) {
+            const int m = bi * 32 + acc_row(4 * g, lane);
+            float v[4];
+            nar_get4(bufA, m, n, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] = (h.c * (acc[4 * g + e] * 0x1p-24f) + h.b * (v[e] * 0x1p-12f) + (m + e == n ? h.a : 0.0f)) * 0x1p11f;
+            nar_put4(bufB, m, n, v);
         }
-        nar_put_symmetric(bufB, bi, bj, lane, acc);
     }
     __syncthreads();
     // 3. the panels
-    f32x16 gram[2] = {};
+    f32x16 gram = {};
     for (int p = first; p < end; p++) {
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-            if (ib + x >= J.nb) continue;
-            const int i0 = (ib + x) * 32, hh = lane >> 5;
+        if (ib < J.nb) {
+            const int i0 = ib * 32, hh = lane >> 5;
             f32x16 acc = {}, cross = {};
             const bool across = LASTSTEP && flip;   // the output's rows are the long index: lanes along the short one
 #pragma unroll
             for (int c = 0; c < 8; c++) {
                 if (c >= steps) continue;
                 const f16x8 bh = nar_frag(bufB, i0 + (lane & 31), c, hh, 0), bl = nar_frag(bufB, i0 + (lane & 31), c, hh, 1);
-                if (across) mul3(acc, cross, t[c][0], t[c][1], bh, bl);
-                else mul3(acc, cross, bh, bl, t[c][0], t[c][1]);
+                f16x8 th, tl;
+                if (c < 4) {
+                    th = t[c & 3][0];
+                    tl = t[c & 3][1];
+                } else {
+                    th = *(const f16x8*)(bufT + ((jb * 4 + c - 4) * 2) * 1024 + lane * 16);
+                    tl = *(const f16x8*)(bufT + ((jb * 4 + c - 4) * 2 + 1) * 1024 + lane * 16);
+                }
+                if (across) mul3(acc, cross, th, tl, bh, bl);
+                else mul3(acc, cross, bh, bl, th, tl);
+                if (c & 1) __builtin_amdgcn_sched_barrier(0);   // 128 registers a wave: not all of B's reads at once
             }
             acc += cross;
             if (!LASTSTEP) {
@@ -504,9 +566,9 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
                         *(f16*)(bufA + nar_off(i, j, 0)) = hi[e];
                         *(f16*)(bufA + nar_off(i, j, 1)) = lo[e];
                     }
-                    const int c = 2 * (ib + x) + half;
-                    *(f16x8*)(nar_t(J.t[cur ^ 1], p, jb, c, 0) + lane * 16) = hi;
-                    *(f16x8*)(nar_t(J.t[cur ^ 1], p, jb, c, 1) + lane * 16) = lo;
+                    const int c = 2 * ib + half;
+                    *(f16x8*)(nar_t(t_next, p, jb, c, 0) + lane * 16) = hi;
+                    *(f16x8*)(nar_t(t_next, p, jb, c, 1) + lane * 16) = lo;
                 }
             } else {
                 const int col = (across ? i0 : p * NPANEL + jb * 32) + (lane & 31), row0 = across ? p * NPANEL + jb * 32 : i0;
@@ -514,8 +576,10 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int row = row0 + acc_row(r, lane);
-                    old[r] = h.update && row < J.rows && col < J.cols ? to_f32(((const T*)J.w)[(i64)row * J.cols + col]) : 0.0f;
+                    const bool in = row < J.rows && col < J.cols;
+                    old[r] = to_f32(((const T*)J.w)[in && h.update ? (i64)row * J.cols + col : 0]);
                 }
+                loads_first();
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int row = row0 + acc_row(r, lane);
@@ -526,14 +590,17 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
                 }
             }
         }
-        if (p + 1 < end) fetch(p + 1);
-        if (!LASTSTEP) {
-            __syncthreads();
-            nar_gram(J, bufA, wave, lane, gram);
-            __syncthreads();
+        if (LASTSTEP && p + 1 == end) break;
+        __syncthreads();   // bufT has been read; bufA holds the new panel
+        if (p + 1 < end) {
+            fetch_high(p + 1);
+            fetch(p + 1);
         }
+        if (!LASTSTEP) nar_gram(J, bufA, wave, lane, gram);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
     }
-    if (!LASTSTEP) nar_gram_store(J, J.gram[cur ^ 1], group, wave, lane, gram);
+    if (!LASTSTEP) nar_gram_store(J, group, wave, lane, gram);
 }
 
 // ---------------------------------------------------------------------------------------------------- host side
@@ -564,18 +631,19 @@ static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
         const int panels = (J.l + NPANEL - 1) / NPANEL;
         J.per_group = (panels + MAX_GROUPS - 1) / MAX_GROUPS;
         J.groups = (panels + J.per_group - 1) / J.per_group;
-        for (int i = 0; i < 2; i++) {
-            J.t[i] = take((size_t)panels * NPANEL * NARROW * 4);
-            J.gram[i] = (float*)take((size_t)J.groups * (J.nb * (J.nb + 1) / 2) * 4096);
-        }
+        J.t0 = take((size_t)panels * NPANEL * NARROW * 4);
+        J.t1 = take((size_t)panels * NPANEL * NARROW * 4);
+        J.gram = (float*)take((size_t)J.groups * (J.nb * (J.nb + 1) / 2) * 4096);
+        J.image = take(NBUF);
         J.x = J.a = J.b = nullptr;
         return off;
     }
-    J.gram[0] = J.gram[1] = nullptr;
+    J.gram = nullptr;
+    J.image = nullptr;
     J.groups = J.per_group = 0;
     J.x = take((size_t)J.sp * J.lp * 4);
-    J.t[0] = take((size_t)J.sp * J.lp * 4);
-    J.t[1] = take((size_t)J.sp * J.lp * 4);
+    J.t0 = take((size_t)J.sp * J.lp * 4);
+    J.t1 = take((size_t)J.sp * J.lp * 4);
     J.a = take((size_t)J.sp * J.sp * 4);
     J.b = take((size_t)J.sp * J.sp * 4);
     return off;
@@ -637,11 +705,16 @@ static void product(Jobs& js, const Hyper& h, int cur, hipStream_t st) {
 static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
     each_first(js, [](const Job& J) { return J.n_part; });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
-    each_first(js, [](const Job& J) { return J.groups; });
-    const dim3 grid(js.first[js.n]), block(NTHREADS);
+    int most = 0;
+    for (int i = 0; i < js.n; i++) most = js.j[i].groups > most ? js.j[i].groups : most;
+    const dim3 grid(most, js.n), block(NTHREADS);
     AZ_DISPATCH_DTYPE(dtype, k_narrow_init<T><<<grid, block, NBUF, st>>>(js, h));
-    for (int it = 0; it + 1 < steps; it++) k_narrow_step<float, false><<<grid, block, 2 * NBUF, st>>>(js, h, it & 1);
-    AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true><<<grid, block, 2 * NBUF, st>>>(js, h, (steps - 1) & 1));
+    const dim3 grid_sum(10, js.n);   // blocks of a 128 x 128 matrix's lower triangle
+    for (int it = 0; it < steps; it++) {
+        k_narrow_sum<<<grid_sum, dim3(256), 0, st>>>(js);
+        if (it + 1 < steps) k_narrow_step<float, false><<<grid, block, NSTEP_LDS, st>>>(js, h, it & 1);
+    }
+    AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true><<<grid, block, NSTEP_LDS, st>>>(js, h, (steps - 1) & 1));
     return launch_status("az_orthogonalize");
 }
 
