@@ -1,0 +1,173 @@
+"""The reference's policy/value CNN (environments/Connect4/Network.py:16-85) evaluated in 8-bit integers, at any width, depth,
+number of planes and board: for networks that the fused kernel does not know (az_net_load takes h_dim 128 on the 6 x 7 board).
+
+An object of this class is a policy_value_fn: MCTS_AZ / AlphaZeroPlayer call its predict between az_select and az_backup
+(MCTS.py:145-146), arena.NetworkSide its net_forward.  Weights are quantised once, a scale for each output channel
+(BatchNorm folded in float64); activations anew in every layer, a scale for each board cell (alphazero_amd.int8).
+Each weight is off by at most half of 1/127 of its channel's largest, each activation by half of 1/127 of its row's.
+"""
+import re
+
+import numpy as np
+import torch
+
+from . import int8
+from ._abi import AzError
+
+BN_EPS = 1e-5   # torch.nn.BatchNorm2d's
+
+
+def neighbour_index(rows, cols, boards, device):
+    """int32 [boards * rows * cols, 9]: where the taps of a 3x3 convolution with zero padding come from, -1 outside the board"""
+    r, c = np.divmod(np.arange(rows * cols), cols)
+    taps = []
+    for dr in (-1, 0, 1):
+        for dc in (-1, 0, 1):
+            inside = (r + dr >= 0) & (r + dr < rows) & (c + dc >= 0) & (c + dc < cols)
+            taps.append(np.where(inside, (r + dr) * cols + c + dc, -1))
+    one = torch.from_numpy(np.stack(taps, 1).astype(np.int32)).to(device)
+    base = torch.arange(boards, dtype=torch.int32, device=device).view(-1, 1, 1) * (rows * cols)
+    return torch.where(one >= 0, one + base, one).reshape(-1, 9).contiguous()
+
+
+class Int8CNN:
+    def __init__(self, state_dict, board=(6, 7), device="cuda", dtype=torch.float32, game="Connect4"):
+        """state_dict: of the reference's CNN (or a module that has one).  dtype: of the activations between layers; float32
+        holds whatever a checkpoint does, float16 halves their traffic for networks whose activations stay below 65504."""
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise AzError("Int8CNN: dtype must be float32, float16 or bfloat16")
+        self.device = torch.device(device)
+        if self.device.type != "cuda":
+            raise AzError("Int8CNN runs on the GPU only (no CPU path)")
+        self.board, self.dtype, self.game = (int(board[0]), int(board[1])), dtype, game
+        self.cells = self.board[0] * self.board[1]
+        self._index = {}
+        self.load_state_dict(state_dict.state_dict() if hasattr(state_dict, "state_dict") else state_dict)
+
+    def name(self):
+        return "Int8CNN"
+
+    # the torch module switches (Network.py:67,79); BatchNorm is folded, there is only eval mode
+    def eval(self):
+        return self
+
+    def train(self, mode=True):
+        return self
+
+    # ---- weights
+    def load_state_dict(self, sd):
+        layers = self._read(sd)
+        self.layers = {k: self._quantize(*v) for k, v in layers.items()}     # only when all of it was accepted
+
+    def sync_from(self, module):
+        """the hot reload after a training step: module is the reference's torch CNN (or anything with state_dict())"""
+        self.load_state_dict(module.state_dict())
+
+    def _read(self, sd):
+        """name -> (matrix [out, k] float64, bias [out] float64), BatchNorm folded, k in the order of our rows"""
+        def get(key):
+            if key not in sd:
+                raise AzError("Int8CNN: the state_dict has no %s" % key)
+            t = sd[key].detach().double().cpu()
+            if not torch.isfinite(t).all():
+                raise AzError("Int8CNN: %s holds a non-finite value" % key)
+            return t
+
+        def folded(conv, bn):
+            w, g, b = get(conv + ".weight"), get(bn + ".weight"), get(bn + ".bias")
+            mean, var = get(bn + ".running_mean"), get(bn + ".running_var")
+            if w.dim() != 4 or w.shape[2] != w.shape[3] or w.shape[2] not in (1, 3):
+                raise AzError("Int8CNN: %s is no 1x1 or 3x3 convolution" % conv)
+            k = g / torch.sqrt(var + BN_EPS)
+            w = w * k.view(-1, 1, 1, 1)
+            return w.permute(0, 2, 3, 1).reshape(w.shape[0], -1), b - mean * k      # (tap, input channel)
+
+        out = {"stem": folded("hidden.0", "hidden.1")}
+        blocks = sorted({int(m.group(1)) for m in (re.match(r"hidden\.(\d+)\.conv\.0\.weight$", k) for k in sd) if m})
+        for i, b in enumerate(blocks):
+            out["conv%d" % i] = folded("hidden.%d.conv.0" % b, "hidden.%d.conv.1" % b)
+            out["mix%d" % i] = folded("hidden.%d.conv.4" % b, "hidden.%d.conv.5" % b)
+        for head in ("policy", "value"):
+            out[head + "_conv"] = folded(head + "_head.0", head + "_head.1")
+            w, c = get(head + "_head.4.weight"), out[head + "_conv"][0].shape[0]
+            if w.shape[1] != c * self.cells:
+                raise AzError("Int8CNN: %s_head.4 takes %d values, the board gives %d" % (head, w.shape[1], c * self.cells))
+            w = w.view(-1, c, self.cells).permute(0, 2, 1).reshape(w.shape[0], -1)  # nn.Flatten's (channel, cell) -> (cell, channel)
+            out[head + "_out"] = (w, get(head + "_head.4.bias"))
+        self.n_blocks = len(blocks)
+        self.in_dim = sd["hidden.0.weight"].shape[1]
+        self.h_dim = sd["hidden.0.weight"].shape[0]
+        self.n_actions = out["policy_out"][0].shape[0]
+        return out
+
+    def _quantize(self, w, b):
+        q, s = int8.quantize_rows(w.float().to(self.device).contiguous())
+        return q, s, b.float().to(self.device)
+
+    # ---- inference
+    def _neighbours(self, boards):
+        if boards not in self._index:
+            if len(self._index) >= 8:      # a search asks for a handful of batch sizes
+                self._index.clear()
+            self._index[boards] = neighbour_index(*self.board, boards, self.device)
+        return self._index[boards]
+
+    def _conv3(self, x, name, boards):
+        q, s = int8.quantize_rows(x, index=self._neighbours(boards))
+        w, ws, b = self.layers[name]
+        return int8.matmul(q, s, w, ws, bias=b, act="silu", dtype=self.dtype)
+
+    def _logits(self, x, head, boards):
+        w, ws, b = self.layers[head + "_conv"]
+        t = int8.linear(x, w, ws, bias=b, act="silu")
+        q, s = int8.quantize_rows(t.view(boards, -1))
+        w, ws, b = self.layers[head + "_out"]
+        return int8.matmul(q, s, w, ws, bias=b)
+
+    @torch.no_grad()
+    def forward_device(self, planes):
+        """(logits [B, n_actions], value logits [B, 3]) float32 of planes [B, in_dim, rows, cols], all on the device"""
+        if planes.dim() != 4 or tuple(planes.shape[1:]) != (self.in_dim,) + self.board:
+            raise AzError("Int8CNN: planes must be [B, %d, %d, %d]" % ((self.in_dim,) + self.board))
+        B = planes.shape[0]
+        if B == 0:
+            return (torch.empty(0, self.n_actions, device=self.device), torch.empty(0, self.layers["value_out"][0].shape[0], device=self.device))
+        x = planes.to(self.device, self.dtype).permute(0, 2, 3, 1).reshape(B * self.cells, self.in_dim).contiguous()
+        x = self._conv3(x, "stem", B)
+        for i in range(self.n_blocks):
+            t = self._conv3(x, "conv%d" % i, B)
+            w, ws, b = self.layers["mix%d" % i]
+            x = int8.linear(t, w, ws, bias=b, residual=x, act="silu")
+        return self._logits(x, "policy", B), self._logits(x, "value", B)
+
+    def forward(self, state):
+        """(log_prob (B, n_actions), value_log_prob (B, 3)) float32 numpy -- Network.py:60-64"""
+        p, v = self.forward_device(torch.as_tensor(state))
+        return torch.log_softmax(p, 1).cpu().numpy(), torch.log_softmax(v, 1).cpu().numpy()
+
+    def predict(self, state, draw_factor=0.5):
+        """(probs (B, n_actions), value (B, 1)) float32 numpy, Network.py:78-85: classes [draw, mover wins, mover loses], a draw
+        worth -player * draw_factor (the last plane holds the player to move)"""
+        state = torch.as_tensor(state)
+        p, v = self.forward_device(state)
+        v = torch.softmax(v, 1)
+        player = state[:, -1, 0, 0].to(self.device, torch.float32)
+        value = -player * draw_factor * v[:, 0] + v[:, 1] - v[:, 2]
+        return torch.softmax(p, 1).cpu().numpy(), value.view(-1, 1).cpu().numpy()
+
+    def policy(self, state):
+        return self.predict(state)[0]
+
+    def value(self, state):
+        return np.exp(self.forward(state)[1])
+
+    def net_forward(self, states):
+        """SelfPlayEngine.net_forward's form, of packed positions: (logp, logv, probs, value)"""
+        from .engine import env_planes_batch
+        planes = torch.from_numpy(env_planes_batch(self.game, states, device=self.device.index or 0))
+        p, v = self.forward_device(planes)
+        logp, logv = torch.log_softmax(p, 1), torch.log_softmax(v, 1)
+        w = logv.exp()
+        player = planes[:, -1, 0, 0].to(self.device)
+        value = (-player * 0.5 * w[:, 0] + w[:, 1] - w[:, 2]).view(-1, 1)
+        return logp.cpu().numpy(), logv.cpu().numpy(), logp.exp().cpu().numpy(), value.cpu().numpy()

@@ -77,3 +77,65 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     ws, wsp = workspace(nws, weights[0])
     check(L.az_muon_step_dev(dev, DTYPES[dt], items, n, lr, momentum, 1 if nesterov else 0, weight_decay, steps, _coeffs(coeffs),
                              eps, wsp, nws, stream_of(dev)))
+
+
+class Muon(torch.optim.Optimizer):
+    """torch optimiser around muon_step, for the matrices and convolutions of a network that is trained beside the engine (the
+    reference's Base.train_step calls self.opt, NetworkBase.py:26-62): weights of at least two dimensions, seen as
+    [out, rest].  Biases and norms belong to another optimiser (`matrices_of` tells them apart).  Momenta are float32."""
+
+    def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS, eps=1e-7):
+        if not lr >= 0.0:
+            raise ValueError("Muon: bad lr %r" % (lr,))
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError("Muon: bad momentum %r" % (momentum,))
+        super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
+                                      coeffs=tuple(coeffs), eps=eps))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() < 2 or p.dtype not in DTYPES:
+                del self.param_groups[-1]
+                raise ValueError("Muon takes float32, float16 or bfloat16 weights of at least two dimensions, not %s %s"
+                                 % (tuple(p.shape), p.dtype))
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            lists = {}   # one call for the weights of a device and dtype
+            for p in group["params"]:
+                if p.grad is None or p.numel() == 0:
+                    continue
+                if p.grad.is_sparse:
+                    raise AzError("Muon: sparse gradients are not supported")
+                state = self.state[p]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                w, g, m = lists.setdefault((p.device, p.dtype), ([], [], []))
+                w.append(p.detach())
+                g.append(p.grad.detach().to(p.dtype).contiguous())
+                m.append(state["momentum"])
+            for w, g, m in lists.values():
+                muon_step(w, g, m, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
+                          weight_decay=group["weight_decay"], steps=group["steps"], coeffs=group["coeffs"], eps=group["eps"])
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)   # casts a state to its parameter's dtype; the momenta stay float32
+        saved = state_dict["state"]
+        order = [p for group in self.param_groups for p in group["params"]]
+        names = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for p, i in zip(order, names):
+            if i in saved and "momentum" in saved[i]:
+                self.state[p]["momentum"] = saved[i]["momentum"].detach().to(device=p.device, dtype=torch.float32, copy=True)
+
+
+def matrices_of(module):
+    """(weights for Muon, the other parameters) of a module: of at least two dimensions, or not"""
+    params = [p for p in module.parameters() if p.requires_grad]
+    return [p for p in params if p.dim() >= 2], [p for p in params if p.dim() < 2]
