@@ -485,9 +485,9 @@ static i64 up(i64 n, i64 to) { return (n + to - 1) / to * to; }
 constexpr i64 FEW_ROWS = 64;          // up to this many rows of q: k_i8_mm_few
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
-using Tile256 = TileShape<256, 256, 2, 4, 4>;
-using Tile128 = TileShape<128, 128, 2, 2, 4>;
-using Tile64 = TileShape<64, 64, 2, 2, 4>;
+using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;
+using Tile128 = TileShape<128, 128, 2, 2, 4, 1>;
+using Tile64 = TileShape<64, 64, 2, 2, 4, 1>;
 
 // How a product is computed; a function of the sizes and alignments alone, so that the workspace can be asked for first.
 struct MmPlan {

@@ -186,13 +186,6 @@ __host__ __device__ inline void product_dims(int mode, const Job& J, int& rows, 
     rows = mode == GRAM || mode == POLY ? J.sp : (mode == STEP || flip ? J.lp : J.sp);
     cols = mode == LAST && !flip ? J.lp : J.sp;
 }
-// tiles of a symmetric launch: tile row i covers rows from bm i on and has the tiles whose first column is not behind its last
-// row: (i + 1) bm / bn of them, but for the last row, which ends with the matrix
-__host__ __device__ inline int symmetric_tiles(int n, int bm, int bn) {
-    const int full = n / bm, per = bm / bn;
-    return per * full * (full + 1) / 2 + (n % bm ? (n + bn - 1) / bn : 0);
-}
-
 // the tile's result passes through LDS as float32, so that rows leave it 16 bytes a lane
 template <class S>
 struct Staged {
@@ -218,15 +211,8 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
     else { P = J.b; Q = t_cur; kp = J.sp; }
     u32 tm, tn;
     const int block = blockIdx.x - js.first[ji];
-    if (SYM) {
-        constexpr int PER = S::BM / S::BN;
-        tm = (u32)((sqrtf(8.0f * (float)(block / PER) + 1.0f) - 1.0f) * 0.5f);   // the row i with PER i (i + 1) / 2 <= block
-        while (PER * tm * (tm + 1) / 2 > (u32)block) tm--;
-        while (PER * (tm + 1) * (tm + 2) / 2 <= (u32)block) tm++;
-        tn = block - PER * tm * (tm + 1) / 2;
-    } else {
-        tile_place(block, (rows + S::BM - 1) / S::BM, (cols + S::BN - 1) / S::BN, tm, tn);
-    }
+    if (SYM) symmetric_place(block, (rows + S::BM - 1) / S::BM, S::BM / S::BN, (cols + S::BN - 1) / S::BN, tm, tn);
+    else tile_place(block, (rows + S::BM - 1) / S::BM, (cols + S::BN - 1) / S::BN, tm, tn);
     const int m0 = tm * S::BM, n0 = tn * S::BN;
     const int mrows = rows - m0 < S::BM ? rows - m0 : S::BM, ncols = cols - n0 < S::BN ? cols - n0 : S::BN;
     const TileSrc<false> p(P + m0 * TILE_KB, (u64)rows * TILE_KB, TILE_KB, mrows * TILE_KB, lane);
@@ -284,20 +270,32 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
             split_store8(outT + split_off(n0 + c, cols, m0 + r), v);
         }
     } else {
-        for (int u = tid; u < S::BM * S::BN; u += S::THREADS) {
-            const int r = u / S::BN, c = u % S::BN;
+        // four neighbouring columns a thread; whole and aligned where the matrix's rows are
+        struct __attribute__((aligned(4 * sizeof(T)))) Four { T v[4]; };
+        const bool whole = J.cols % 4 == 0 && ((uintptr_t)J.w & (4 * sizeof(T) - 1)) == 0;
+#pragma unroll 4
+        for (int u = tid; u < S::BM * S::BN / 4; u += S::THREADS) {
+            const int r = u / (S::BN / 4), c = u % (S::BN / 4) * 4;
             if (m0 + r >= J.rows || n0 + c >= J.cols) continue;
-            float o = tile[r * PITCH + c];
+            const f32x4 o = *(const f32x4*)(tile + r * PITCH + c);
             T* w = (T*)J.w + (i64)(m0 + r) * J.cols + n0 + c;
-            if (h.update) o = to_f32(*w) * h.decay - o * (h.lr * J.kappa);
-            *w = from_f32<T>(o);
+            if (whole) {
+                Four f;
+                if (h.update) f = *(const Four*)w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) f.v[e] = from_f32<T>(h.update ? to_f32(f.v[e]) * h.decay - o[e] * (h.lr * J.kappa) : o[e]);
+                *(Four*)w = f;
+            } else {
+                for (int e = 0; e < 4 && n0 + c + e < J.cols; e++)
+                    w[e] = from_f32<T>(h.update ? to_f32(w[e]) * h.decay - o[e] * (h.lr * J.kappa) : o[e]);
+            }
         }
     }
 }
 
-using OTile128 = TileShape<128, 128, 2, 2, 4>;
-using OTile128s = TileShape<128, 64, 2, 2, 4>;   // symmetric results
-using OTile64 = TileShape<64, 64, 2, 2, 4>;
+using OTile128 = TileShape<128, 128, 2, 2, 4, 1>;
+using OTile128s = TileShape<128, 64, 2, 2, 4, 1>;   // symmetric results
+using OTile64 = TileShape<64, 64, 2, 2, 3, 4>;   // few tiles: what counts is the way from step to step, so few barriers
 
 // ---------------------------------------------------------------------------------------------------- Narrow matrices
 // Short side s <= 128: two launches a step.  B (s x s) fits LDS, and so does a panel of 128 values of the long index.  The first
@@ -677,7 +675,8 @@ static int product_blocks(Jobs& js) {   // fills js.first
     each_first(js, [](const Job& J) {
         int rows, cols;
         product_dims(MODE, J, rows, cols);
-        if (MODE == GRAM || MODE == POLY) return (i64)symmetric_tiles(J.sp, S::BM, S::BN);
+        if (MODE == GRAM || MODE == POLY)
+            return (i64)symmetric_total((rows + S::BM - 1) / S::BM, S::BM / S::BN, (cols + S::BN - 1) / S::BN);
         return (i64)((rows + S::BM - 1) / S::BM) * ((cols + S::BN - 1) / S::BN);
     });
     return js.first[js.n];

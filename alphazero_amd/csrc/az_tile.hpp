@@ -121,20 +121,24 @@ __device__ inline void step_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
 }
 
-// a workgroup's tile: BM x BN outputs, WM x WN waves
-template <int BM_, int BN_, int WM_, int WN_, int STAGES_>
+// a workgroup's tile: BM x BN outputs, WM x WN waves, STAGES buffers of GROUP steps each (a barrier every GROUP steps)
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int GROUP_>
 struct TileShape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, STAGES = STAGES_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, WAVES = WM * WN, THREADS = 64 * WAVES, STAGES = STAGES_, GROUP = GROUP_;
     static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;
     static constexpr bool PAIRS = FN % 2 == 0;   // lane c of blocks 2 j and 2 j + 1: columns 64 j + 2 c, 64 j + 2 c + 1
-    static constexpr int STEP_BYTES = (BM + BN) * TILE_KB, LDS = STAGES * STEP_BYTES;
+    static constexpr int STEP_BYTES = (BM + BN) * TILE_KB, STAGE_BYTES = GROUP * STEP_BYTES, LDS = STAGES * STAGE_BYTES;
     static_assert(LDS <= 160 * 1024 && STAGES >= 2, "the ring fits LDS");
 };
 
+// GROUP steps from `step` on into the buffer at `stage`
 template <class S>
-__device__ inline void step_load(const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 step, u32 kend, u8* tile, int wave) {
-    tile_load<S::BM, S::WAVES, false>(p, step, kend, tile, wave);
-    tile_load<S::BN, S::WAVES, S::PAIRS>(q, step, kend, tile + S::BM * TILE_KB, wave);
+__device__ inline void stage_load(const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 step, u32 kend, u8* stage, int wave) {
+#pragma unroll
+    for (int g = 0; g < S::GROUP; g++) {
+        tile_load<S::BM, S::WAVES, false>(p, step + g, kend, stage + g * S::STEP_BYTES, wave);
+        tile_load<S::BN, S::WAVES, S::PAIRS>(q, step + g, kend, stage + g * S::STEP_BYTES + S::BM * TILE_KB, wave);
+    }
 }
 
 // The order of a slice's instructions: its reads spread over its MFMAs from the first one on (left alone, the compiler moves the
@@ -149,48 +153,49 @@ __device__ inline void spread_reads() {
     }
 }
 
-// The steps from `step` up to byte kend of the rows, kend a multiple of 16 (whole steps are read, with zeros behind kend).
-// One barrier a step: it says that the next step's tiles have landed and that everybody holds this step's last slice in
-// registers.  That slice is multiplied behind it, while the next step's first slice is on its way from LDS and the step STAGES
+// The steps from `at` up to byte kend of the rows, kend a multiple of 16 (whole groups are read, with zeros behind kend).
+// One barrier a group of steps: it says that the next group's tiles have landed and that everybody holds this group's last slice
+// in registers.  That slice is multiplied behind it, while the next group's first slice is on its way from LDS and the group STAGES
 // ahead (into the buffer that has just become free) on its way from memory.  Behind the last step the loads ask for nothing
 // (zeros) and the slice read is nobody's: no branch in the loop, and the count of loads in flight stays what the barrier waits for.
 template <class Kind, class S>
 __device__ inline void tile_product(Kind, const TileSrc<false>& p, const TileSrc<S::PAIRS>& q, u32 at, u32 kend, u8* lds, int wave,
                                     int lane, typename Kind::acc_t (&acc)[S::FM][S::FN]) {
     const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32);
-    constexpr int LOADS = S::BM / (16 * S::WAVES) + S::BN / (16 * S::WAVES), KS = Kind::KS, Q = S::BM * TILE_KB;
+    constexpr int LOADS = S::GROUP * (S::BM + S::BN) / (16 * S::WAVES), KS = Kind::KS, Q = S::BM * TILE_KB, SL = S::GROUP * KS;
+    static_assert((S::STAGES - 1) * LOADS < 64, "vmcnt counts to 63");
     typedef typename Kind::template Slice<S::FM, S::FN> Slice;
 #pragma unroll
-    for (int s = 0; s < S::STAGES; s++) step_load<S>(p, q, at + s, kend, lds + s * S::STEP_BYTES, wave);
+    for (int s = 0; s < S::STAGES; s++) stage_load<S>(p, q, at + s * S::GROUP, kend, lds + s * S::STAGE_BYTES, wave);
     step_barrier<(S::STAGES - 1) * LOADS>();
     Slice f0, f1;
     f0.read(lds, lds + Q, wm, wn, 0, lane);
     u8* cur = lds;
-    auto step = [&](Slice& first, Slice& other) {   // first: holds the step's slice 0; afterwards the next step's is in...
-        u8* nxt = cur + S::STEP_BYTES < lds + S::LDS ? cur + S::STEP_BYTES : lds;
-        if constexpr (KS == 2) {
-            other.read(cur, cur + Q, wm, wn, 1, lane);
-            first.mul(acc);
+    auto group = [&](Slice& even, Slice& odd) {   // even: holds slice 0; odd is free
+        u8* nxt = cur + S::STAGE_BYTES < lds + S::LDS ? cur + S::STAGE_BYTES : lds;
+#pragma unroll
+        for (int sl = 0; sl + 1 < SL; sl++) {
+            u8* step = cur + (sl + 1) / KS * S::STEP_BYTES;
+            (sl & 1 ? even : odd).read(step, step + Q, wm, wn, (sl + 1) % KS, lane);
+            (sl & 1 ? odd : even).mul(acc);
             spread_reads<Kind::READS * (S::FM + S::FN), Kind::MULS * S::FM * S::FN>();
             __builtin_amdgcn_sched_barrier(0);
         }
         step_barrier<(S::STAGES - 2) * LOADS>();
-        Slice& last = KS == 2 ? other : first;
-        Slice& next = KS == 2 ? first : other;      // ... `first` (two slices a step) or `other` (one)
-        next.read(nxt, nxt + Q, wm, wn, 0, lane);
-        step_load<S>(p, q, at + S::STAGES, kend, cur, wave);
-        last.mul(acc);
+        (SL & 1 ? odd : even).read(nxt, nxt + Q, wm, wn, 0, lane);
+        stage_load<S>(p, q, at + S::STAGES * S::GROUP, kend, cur, wave);
+        (SL & 1 ? even : odd).mul(acc);
         __builtin_amdgcn_sched_barrier(0);
         cur = nxt;
-        at++;
+        at += S::GROUP;
     };
     const u32 end = (kend + TILE_KB - 1) / TILE_KB;
-    if constexpr (KS == 2) {
-        while (at < end) step(f0, f1);
+    if constexpr (SL % 2 == 0) {
+        while (at < end) group(f0, f1);
     } else {
-        while (at < end) {   // a step behind the last multiplies zeros (leaving in the middle would copy the accumulators)
-            step(f0, f1);
-            step(f1, f0);
+        while (at < end) {   // a group behind the last multiplies zeros (leaving in the middle would copy the accumulators)
+            group(f0, f1);
+            group(f1, f0);
         }
     }
     step_barrier<0>();   // nothing is on its way into LDS any more
@@ -199,13 +204,39 @@ __device__ inline void tile_product(Kind, const TileSrc<false>& p, const TileSrc
 // Which tile a workgroup computes.  Workgroups go to the 8 XCDs in turn and every XCD has its own L2: each XCD gets a
 // contiguous run of tiles, and runs go through the tiles in bands of 8 tile rows, column by column, so that the tiles in
 // flight on an XCD share few rows of P and Q.
+__host__ __device__ inline u32 xcd_run(u32 block, u32 total) {
+    const u32 per = total / 8, rest = total % 8, x = block & 7, i = block >> 3;
+    return x * per + (x < rest ? x : rest) + i;   // XCD x has `per` tiles, one more if x < rest
+}
 __device__ inline void tile_place(u32 block, u32 tiles_m, u32 tiles_n, u32& tm, u32& tn) {
-    const u32 total = tiles_m * tiles_n, per = total / 8, rest = total % 8, x = block & 7, i = block >> 3;
-    // XCD x has per tiles, one more if x < rest
-    const u32 t = x * per + (x < rest ? x : rest) + i;
+    const u32 t = xcd_run(block, tiles_m * tiles_n);
     const u32 band = t / (8 * tiles_n), first = band * 8, rows = tiles_m - first < 8 ? tiles_m - first : 8, in = t - band * 8 * tiles_n;
     tm = first + in % rows;
     tn = in / rows;
+}
+
+// The same for the tiles of a symmetric matrix that touch its lower triangle: rows of bm = `per` bn, row i has the first
+// min(per (i + 1), cols) tiles.  Bands of 4 rows, column by column.
+__host__ __device__ inline u32 symmetric_row(u32 i, u32 per, u32 cols) { return per * (i + 1) < cols ? per * (i + 1) : cols; }
+__host__ __device__ inline u32 symmetric_total(u32 rows, u32 per, u32 cols) {
+    return per * (rows - 1) * rows / 2 + symmetric_row(rows - 1, per, cols);
+}
+__host__ __device__ inline void symmetric_place(u32 block, u32 rows, u32 per, u32 cols, u32& tm, u32& tn) {
+    u32 t = xcd_run(block, symmetric_total(rows, per, cols));
+    for (u32 r0 = 0;; r0 += 4) {
+        const u32 nr = rows - r0 < 4 ? rows - r0 : 4;
+        u32 from = 0;   // columns before row r0 + k's own: rows r0 + k .. r0 + nr - 1 have them
+        for (u32 k = 0; k < nr; k++) {
+            const u32 to = symmetric_row(r0 + k, per, cols), n = (nr - k) * (to - from);
+            if (t < n) {
+                tm = r0 + k + t % (nr - k);
+                tn = from + t / (nr - k);
+                return;
+            }
+            t -= n;
+            from = to;
+        }
+    }
 }
 
 }  // namespace az
