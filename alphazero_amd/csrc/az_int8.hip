@@ -311,9 +311,19 @@ struct Mm {
     bool pair_store;   // every even column of y starts at a multiple of two elements
 };
 
+template <class T>
 __device__ inline float activate(float v, int act) {
     if (act == AZ_ACT_RELU) return v > 0 || v != v ? v : 0.0f;
-    if (act == AZ_ACT_SILU) return v / (1.0f + expf(-v));
+    if (act == AZ_ACT_SILU) {
+        // For 16-bit results exp2 and rcp of the hardware (2^-22 each, and |v| 2^-24 from the exponent's rounding: far below the
+        // 2^-12 of the result's own rounding wherever it is not vanishing): 6 instructions for the 35 of expf and the division,
+        // which cost a 128 x 128 tile 4 us.
+        if (sizeof(T) == 2) {
+            const float e = __builtin_amdgcn_exp2f(v * -1.44269504088896340736f);
+            return e == __builtin_inff() ? v * 0.0f : v * __builtin_amdgcn_rcpf(1.0f + e);
+        }
+        return v / (1.0f + expf(-v));
+    }
     return v;
 }
 
@@ -331,10 +341,10 @@ __device__ inline u32x4 load_piece(const i8* row, i64 k, i64 K) {
 }
 
 template <class T>
-__device__ inline void put(const Mm& p, i64 m, i64 n, int sum) {
-    float v = (float)sum * p.qs[m] * p.ws[n] + (p.bias ? p.bias[n] : 0.0f);
+__device__ inline void put(const Mm& p, i64 m, i64 n, int sum, float scale) {
+    float v = (float)sum * scale * p.ws[n] + (p.bias ? p.bias[n] : 0.0f);
     if (p.res) v += to_f32(((const T*)p.res)[m * p.ld_res + n]);
-    ((T*)p.y)[m * p.ld_y + n] = from_f32<T>(activate(v, p.act));
+    ((T*)p.y)[m * p.ld_y + n] = from_f32<T>(activate<T>(v, p.act));
 }
 
 // Rows of both operands at multiples of 16 bytes, k a multiple of 16.  blockIdx.y: which of the `splits` parts of k (whole
@@ -399,13 +409,13 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
                         v0 += to_f32(r[0]);
                         if (two) v1 += to_f32(r[1]);
                     }
-                    v0 = activate(v0, p.act);
+                    v0 = activate<T>(v0, p.act);
                     if (two && p.pair_store) {
                         struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
-                        *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate(v1, p.act))};
+                        *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate<T>(v1, p.act))};
                     } else {
                         y[0] = from_f32<T>(v0);
-                        if (two) y[1] = from_f32<T>(activate(v1, p.act));
+                        if (two) y[1] = from_f32<T>(activate<T>(v1, p.act));
                     }
                 }
             }
@@ -417,7 +427,7 @@ __global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __
     for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
         int sum = 0;
         for (u32 s = 0; s < splits; s++) sum += part[s * total + e];
-        put<T>(p, e / p.n, e % p.n, sum);
+        put<T>(p, e / p.n, e % p.n, sum, p.qs[e / p.n]);
     }
 }
 
@@ -465,12 +475,106 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_mm_few(Mm p) {
         int sum = 0;
 #pragma unroll
         for (int i = 0; i < FEW_WAVES; i++) sum += sums[i][m][c];
-        put<T>(p, m, n0 + c, sum);
+        put<T>(p, m, n0 + c, sum, p.qs[m]);
     }
 }
 
-// Rows of k bytes at any address -> rows of kp (a multiple of 16) with zeros behind k.  16 output bytes a thread.
-__global__ __launch_bounds__(256) void k_i8_align(const i8* __restrict__ src, i64 ld, i64 rows, i64 k, i64 kp, i8* __restrict__ dst) {
+// A linear layer on one to four rows: k_i8_mm_few with the rows quantised by every workgroup for itself (they are small beside its
+// 16 rows of w, which it asks for first), instead of a launch that the other waits for.
+constexpr int LIN_ROWS = 4, LIN_AHEAD = 8, LIN_LDS = 64 * 1024;
+template <class T>
+__global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T* __restrict__ x, i64 ld_x) {
+    extern __shared__ __attribute__((aligned(16))) u8 lds[];   // m rows of kp integers
+    __shared__ u32 part[LIN_ROWS][FEW_WAVES];
+    __shared__ int sums[FEW_WAVES][LIN_ROWS][17];
+    constexpr int EPP = Piece<T>::EPP, THREADS = 64 * FEW_WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 15, quarter = lane >> 4, m = (int)p.m;
+    const i64 n0 = (i64)blockIdx.x * 16, n = n0 + row < p.n ? n0 + row : p.n - 1;
+    const i8* w = p.w + n * p.ld_w;
+    const i64 whole = p.k & ~(i64)63;
+    const int k = (int)p.k, kp = (k + 63) & ~63, pieces = (k + EPP - 1) / EPP;
+    i32x4 b[LIN_AHEAD];
+#pragma unroll
+    for (int i = 0; i < LIN_AHEAD; i++) {   // steps that are not there: the row's beginning again (k >= 64 or nothing is loaded)
+        const i64 at = (wave + i * FEW_WAVES) * 64;
+        b[i] = i32x4{0, 0, 0, 0};
+        if (whole) __builtin_memcpy(&b[i], w + (at < whole ? at : 0) + quarter * 16, 16);
+    }
+    u32 mx[LIN_ROWS];
+#pragma unroll
+    for (int r = 0; r < LIN_ROWS; r++) {
+        mx[r] = 0;
+        if (r < m)
+            for (int i = tid; i < pieces; i += THREADS) {
+                Piece<T> v;
+                v.load(x + r * ld_x + (i64)i * EPP, k - i * EPP < EPP ? k - i * EPP : EPP);
+                const u32 t = v.most();
+                mx[r] = t > mx[r] ? t : mx[r];
+            }
+        mx[r] = lanes_max<64>(mx[r]);
+        if (lane == 0) part[r][wave] = mx[r];
+    }
+    __syncthreads();
+    float s[LIN_ROWS];
+#pragma unroll
+    for (int r = 0; r < LIN_ROWS; r++) {
+#pragma unroll
+        for (int i = 0; i < FEW_WAVES; i++) mx[r] = part[r][i] > mx[r] ? part[r][i] : mx[r];
+        s[r] = row_scale(mx[r]);
+        if (r >= m) continue;
+        const float rs = 1.0f / s[r];
+        for (int i = tid; i < kp / EPP; i += THREADS) {   // zeros behind the row
+            u32 out[EPP / 4] = {};
+            if (i < pieces && s[r] > 0) {
+                Piece<T> v;
+                v.load(x + r * ld_x + (i64)i * EPP, k - i * EPP < EPP ? k - i * EPP : EPP);
+                if (!(s[r] >= QUANT_TINY && v.quantize(rs, out))) v.quantize_exact(s[r], rs, out);
+            }
+            __builtin_memcpy(lds + r * kp + i * EPP, out, EPP);
+        }
+    }
+    __syncthreads();
+    const u8* q = lds + (row < m ? row : m - 1) * kp + quarter * 16;
+    i32x4 acc = {};
+#pragma unroll
+    for (int i = 0; i < LIN_AHEAD; i++) {
+        const i64 at = (wave + i * FEW_WAVES) * 64;
+        if (at < whole) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(q + at), b[i], acc, 0, 0, 0);
+    }
+#pragma unroll 4
+    for (i64 at = (wave + LIN_AHEAD * FEW_WAVES) * 64; at < whole; at += FEW_WAVES * 64) {
+        i32x4 v;
+        __builtin_memcpy(&v, w + at + quarter * 16, 16);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(q + at), v, acc, 0, 0, 0);
+    }
+    if (whole < p.k && wave == (int)(whole / 64 % FEW_WAVES))
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(q + whole),
+                                                    __builtin_bit_cast(i32x4, load_piece(w, whole + quarter * 16, p.k)), acc, 0, 0, 0);
+    if (quarter == 0)   // rows 4 quarter + r
+#pragma unroll
+        for (int r = 0; r < 4; r++) sums[wave][r][row] = acc[r];
+    __syncthreads();
+    if (tid < LIN_ROWS * 16) {
+        const int r = tid >> 4, c = tid & 15;
+        if (r >= m || n0 + c >= p.n) return;
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < FEW_WAVES; i++) sum += sums[i][r][c];
+        put<T>(p, r, n0 + c, sum, r == 0 ? s[0] : r == 1 ? s[1] : r == 2 ? s[2] : s[3]);
+    }
+}
+
+// Rows of k bytes at any address -> rows of kp (a multiple of 16) with zeros behind k.  16 output bytes a thread; blockIdx.y: which
+// operand.
+struct Align {
+    const i8* src[2];
+    i64 ld[2], rows[2];
+    i8* dst[2];
+};
+__global__ __launch_bounds__(256) void k_i8_align(Align a, i64 k, i64 kp) {
+    const i8* src = blockIdx.y ? a.src[1] : a.src[0];
+    i8* dst = blockIdx.y ? a.dst[1] : a.dst[0];
+    const i64 ld = blockIdx.y ? a.ld[1] : a.ld[0], rows = blockIdx.y ? a.rows[1] : a.rows[0];
     const i64 pieces = kp / 16, total = rows * pieces;
     for (i64 e = (i64)blockIdx.x * 256 + threadIdx.x; e < total; e += (i64)gridDim.x * 256) {
         const i64 r = e / pieces, c = (e - r * pieces) * 16;
@@ -486,8 +590,8 @@ constexpr i64 FEW_ROWS = 64;          // up to this many rows of q: k_i8_mm_few
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
 using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;
-using Tile128 = TileShape<128, 128, 2, 2, 4, 1>;
-using Tile64 = TileShape<64, 64, 2, 2, 4, 1>;
+using Tile128 = TileShape<128, 128, 4, 2, 3, 1>;   // 48 KB: three workgroups a CU, whose stores run under each other's loads
+using Tile64 = TileShape<64, 64, 2, 2, 3, 2>;
 
 // How a product is computed; a function of the sizes and alignments alone, so that the workspace can be asked for first.
 struct MmPlan {
@@ -513,10 +617,11 @@ static MmPlan mm_plan(i64 m, i64 n, i64 k, const void* q, i64 ld_q, bool q_padde
     // a larger tile reads less per product, but must not be mostly padding and must fill the chip
     auto pays = [&](i64 e) { return tiles(e) >= 200 && tiles(e) * e * e <= tiles(e / 2) * (e / 2) * (e / 2) * 9 / 8; };
     P.tile = pays(256) ? 256 : pays(128) ? 128 : 64;
+    // k split over workgroups where the tiles are too few for the CUs, in parts of at least 16 steps (a join costs 5 us)
     const u32 steps = (u32)((k + TILE_KB - 1) / TILE_KB);
     u32 splits = 1;
     if (P.tile == 64)
-        while (splits < 16 && tiles(64) * splits * 2 <= 512 && steps / (splits * 2) >= 4) splits *= 2;
+        while (splits < 16 && tiles(64) * splits * 2 <= 256 && steps / (splits * 2) >= 16) splits *= 2;
     P.steps_per_split = (steps + splits - 1) / splits;
     P.splits = (steps + P.steps_per_split - 1) / P.steps_per_split;
     P.part_bytes = P.splits > 1 ? up256((size_t)P.splits * m * n * 4) : 0;
@@ -527,14 +632,6 @@ template <class T, class S>
 static int launch_tile(const Mm& p, const MmPlan& P, int* part, hipStream_t st) {
     const i64 tm = (p.m + S::BM - 1) / S::BM, tn = (p.n + S::BN - 1) / S::BN;
     if (tm * tn > 0x7fffffff) return refuse("az_i8_matmul: more than 2^31 tiles");
-    if (S::LDS > 64 * 1024) {
-        hipError_t e = hipFuncSetAttribute((const void*)k_i8_mm_tile<T, S>, hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS);
-        if (e != hipSuccess) {
-            (void)hipGetLastError();
-            set_error("az_i8_matmul: hipFuncSetAttribute failed");
-            return AZ_ERR_HIP;
-        }
-    }
     k_i8_mm_tile<T, S><<<dim3((u32)(tm * tn), P.splits), dim3(S::THREADS), S::LDS, st>>>(p, (u32)tm, (u32)tn, P.steps_per_split, part);
     if (part) {
         const i64 blocks = (p.m * p.n + 255) / 256;
@@ -555,14 +652,25 @@ static int mm_launch(Mm p, const MmPlan& P, char* ws, hipStream_t st) {
         else k_i8_mm_few<T, 4><<<grid, block, 0, st>>>(p);
         return launch_status("az_i8_matmul");
     }
-    auto align = [&](const i8*& src, i64& ld, i64 rows, char* dst) {
-        const i64 blocks = (rows * (P.kp / 16) + 255) / 256;
-        k_i8_align<<<dim3((u32)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, st>>>(src, ld, rows, p.k, P.kp, (i8*)dst);
-        src = (const i8*)dst;
-        ld = P.kp;
-    };
-    if (P.align_q) align(p.q, p.ld_q, p.m, ws);
-    if (P.align_w) align(p.w, p.ld_w, p.n, ws + P.q_bytes);
+    if (P.align_q || P.align_w) {
+        Align a = {};
+        int n = 0;
+        i64 most = 0;
+        auto add = [&](const i8*& src, i64& ld, i64 rows, char* dst) {
+            a.src[n] = src;
+            a.ld[n] = ld;
+            a.rows[n] = rows;
+            a.dst[n] = (i8*)dst;
+            src = (const i8*)dst;
+            ld = P.kp;
+            most = rows > most ? rows : most;
+            n++;
+        };
+        if (P.align_q) add(p.q, p.ld_q, p.m, ws);
+        if (P.align_w) add(p.w, p.ld_w, p.n, ws + P.q_bytes);
+        const i64 blocks = (most * (P.kp / 16) + 255) / 256;
+        k_i8_align<<<dim3((u32)(blocks < 8192 ? blocks : 8192), n), dim3(256), 0, st>>>(a, p.k, P.kp);
+    }
     p.k = P.kp;   // from here on with the zeros (of one operand at least) behind the end
     int* part = P.splits > 1 ? (int*)(ws + P.q_bytes + P.w_bytes) : nullptr;
     if (P.tile == 256) return launch_tile<T, Tile256>(p, P, part, st);
@@ -689,8 +797,10 @@ int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t* 
     return i8_matmul(p, false, dtype, ws_dev, (hipStream_t)stream);
 }
 
+static bool linear_fused(i64 m, i64 k) { return m <= LIN_ROWS && m * up(k, 64) <= LIN_LDS; }
+
 size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k, const int8_t* w_dev, int64_t ld_w) {
-    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K) return 0;
+    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K || linear_fused(m, k)) return 0;
     return up256((size_t)m * linear_pitch(k)) + up256((size_t)m * 4) +
            mm_plan(m, n, k, nullptr, linear_pitch(k), true, w_dev, ld_w).total();
 }
@@ -708,6 +818,14 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void* x_
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || m == 0 || n == 0) return dev.rc;
     hipStream_t st = (hipStream_t)stream;
+    if (linear_fused(m, k)) {
+        const Mm p = {m, n, k, nullptr, w_dev, 0, ld_w, nullptr, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act, false};
+        const i64 blocks = (n + 15) / 16;
+        if (blocks > 0x7fffffff) return refuse("az_i8_linear: more than 2^31 tiles");
+        AZ_DISPATCH_DTYPE(dtype, k_i8_linear_few<T><<<dim3((u32)blocks), dim3(64 * FEW_WAVES), (size_t)(m * up(k, 64)), st>>>(
+                                     p, (const T*)x_dev, ld_x));
+        return launch_status("az_i8_linear");
+    }
     i8* q = (i8*)ws_dev;
     float* qs = (float*)((char*)ws_dev + up256((size_t)m * linear_pitch(k)));
     char* rest = (char*)qs + up256((size_t)m * 4);

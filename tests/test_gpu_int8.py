@@ -189,7 +189,8 @@ def test_matmul_residual_in_place_and_nan(I8):
 
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 1000, 4096), (1, 257, 1031), (2, 64, 100), (3, 7, 42), (4, 300, 4096), (8, 128, 1152),
-                                   (16, 100, 5000), (33, 65, 130), (200, 300, 1031), (1, 33, 131071)])
+                                   (16, 100, 5000), (33, 65, 130), (200, 300, 1031), (1, 33, 131071),
+                                   (2, 17, 32000), (3, 40, 21845), (4, 16, 16384), (4, 100, 63), (5, 9, 64), (1, 5, 65472), (1, 5, 65600)])
 def test_linear_is_quantize_then_matmul(I8, dt, m, n, k):
     g = torch.Generator().manual_seed(m * 7 + n + k)
     x = torch.randn(m, k, generator=g).to(DT[dt]).cuda()
@@ -201,7 +202,7 @@ def test_linear_is_quantize_then_matmul(I8, dt, m, n, k):
     check_layer(y, *layer64(torch.from_numpy(q64), torch.from_numpy(s64), w, ws, b, r, "silu"))
 
 
-@pytest.mark.parametrize("m", [1, 3, 40])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 40])
 def test_linear_non_finite_rows(I8, m):
     x = torch.randn(m, 200).cuda()
     x[0, 13] = float("inf")

@@ -63,8 +63,8 @@ def test_matmul_refuses():
         _refused(call(fn, x=None), "null")
         _refused(call(fn, w=None), "null")
         _refused(call(fn, y=None), "null")
-    _refused(call("linear", nws=16), "workspace")
-    _refused(call("linear", ws=C.c_void_p(264)), "workspace")
+    _refused(call("linear", m=40, nws=16), "workspace")
+    _refused(call("linear", m=40, ws=C.c_void_p(264)), "workspace")
     _refused(call("matmul", m=100, k=7, nws=16), "workspace")          # rows that have to be aligned first
     _refused(call("matmul", m=100, k=7, ws=C.c_void_p(264)), "workspace")
     assert L.az_i8_linear_ws(4, 6, 0, P, 8) == 0 and L.az_i8_matmul_ws(4, 6, 8, P, 8, P, 8) == 0
