@@ -237,14 +237,16 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
     __syncthreads();
     if (MODE != LAST) {   // mrows and ncols are multiples of 64 here
         u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : t_next;
-        // pairs of lanes store 16 values of a row, 64 bytes; the next pair those of the next row, right behind them
+        // 32 lanes store 16 values of 16 rows, 1 KB in a run: 16 lanes the first eight, 16 the others (16 rows read from LDS at
+        // one column are on different banks)
+#pragma unroll 2
         for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
-            const int r = u / 2 % S::BM, c = (u % 2 + u / (2 * S::BM) * 2) * 8, m = m0 + r, n = n0 + c;
+            const int at = u % (2 * S::BM), r = at / 32 * 16 + at % 16, c = u / (2 * S::BM) * 16 + at / 16 % 2 * 8, m = m0 + r, n = n0 + c;
             if (r >= mrows || c >= ncols) continue;
             float v[8];
             float* d = tile + r * PITCH + c;
-#pragma unroll
-            for (int e = 0; e < 8; e++) v[e] = d[e];
+            *(f32x4*)v = *(const f32x4*)d;
+            *(f32x4*)(v + 4) = *(const f32x4*)(d + 4);
             if (MODE == POLY) {
                 float A[8];
                 split_load8(J.a + split_off(m, J.sp, n), A);
@@ -261,6 +263,7 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
         if (SYM && n0 + S::BN > m0) return;
         if (MODE == POLY) __syncthreads();
         u8* outT = MODE == STEP ? J.x : out;
+#pragma unroll 2
         for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
             const int c = u / 2 % S::BN, r = (u % 2 + u / (2 * S::BN) * 2) * 8;
             if (r >= mrows || c >= ncols) continue;
