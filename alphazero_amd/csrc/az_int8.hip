@@ -479,9 +479,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_mm_few(Mm p) {
     }
 }
 
-// A linear layer on one to four rows: k_i8_mm_few with the rows quantised by every workgroup for itself (they are small beside its
-// 16 rows of w, which it asks for first), instead of a launch that the other waits for.
-constexpr int LIN_ROWS = 4, LIN_AHEAD = 8, LIN_LDS = 64 * 1024;
+// A linear layer on one or two rows of up to 16384: k_i8_mm_few with the rows quantised by every workgroup for itself (they are small
+// beside its 16 rows of w, which it asks for first), instead of a launch that the other waits for (us, one launch | two:
+// 1 x 4096 x 4096 6.9 | 8.8, 2 x 4096 x 4096 7.8 | 8.9, 1 x 4096 x 16384 19.1 | 21.3, 1 x 128 x 1152 4.8 | 6.7; four rows 10.9 | 9.7).
+constexpr int LIN_ROWS = 2, LIN_AHEAD = 8, LIN_LDS = 16 * 1024;
 template <class T>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T* __restrict__ x, i64 ld_x) {
     extern __shared__ __attribute__((aligned(16))) u8 lds[];   // m rows of kp integers
@@ -552,7 +553,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T*
                                                     __builtin_bit_cast(i32x4, load_piece(w, whole + quarter * 16, p.k)), acc, 0, 0, 0);
     if (quarter == 0)   // rows 4 quarter + r
 #pragma unroll
-        for (int r = 0; r < 4; r++) sums[wave][r][row] = acc[r];
+        for (int r = 0; r < LIN_ROWS; r++) sums[wave][r][row] = acc[r];
     __syncthreads();
     if (tid < LIN_ROWS * 16) {
         const int r = tid >> 4, c = tid & 15;
@@ -560,7 +561,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T*
         int sum = 0;
 #pragma unroll
         for (int i = 0; i < FEW_WAVES; i++) sum += sums[i][r][c];
-        put<T>(p, r, n0 + c, sum, r == 0 ? s[0] : r == 1 ? s[1] : r == 2 ? s[2] : s[3]);
+        put<T>(p, r, n0 + c, sum, r ? s[1] : s[0]);
     }
 }
 
@@ -586,7 +587,16 @@ static bool pairs_ok(const void* y, i64 ld_y, int dtype) { return ld_y % 2 == 0 
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static i64 up(i64 n, i64 to) { return (n + to - 1) / to * to; }
 
-constexpr i64 FEW_ROWS = 64;          // up to this many rows of q: k_i8_mm_few
+// When k_i8_mm_few takes a product of up to 64 rows.  It reads q from L2 once for every 16 channels, the tiles once for every 64, and
+// splits k over 8 waves only, the tiles over 16 workgroups; but it is one launch and takes rows at any address, which the tiles
+// need copied first (us, few | tiles: 1 x 4096 x 4096 5.0 | 8.4, 16 x 4096 x 4096 6.4 | 9.4, 16 x 8192 x 8192 17.5 | 16.2,
+// 16 x 128 x 16384 16.1 | 10.9, 32 x 4096 x 4096 8.3 | 10.3, 32 x 8192 x 8192 24.8 | 17.4, 42 x 128 x 1152 4.5 | 7.2,
+// 64 x 1024 x 1024 5.0 | 7.2, 64 x 4096 x 4096 12.1 | 11.2, 64 x 8192 x 8192 38.7 | 18.7).
+static bool few_rows(i64 m, i64 n, i64 k, bool aligned) {
+    if (m > 64) return false;
+    if (!aligned) return true;
+    return k <= 8192 && (m <= 16 || n * k <= (m <= 32 ? 16 << 20 : 8 << 20));
+}
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
 using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;
@@ -607,17 +617,20 @@ static MmPlan mm_plan(i64 m, i64 n, i64 k, const void* q, i64 ld_q, bool q_padde
     MmPlan P = {};
     P.splits = 1;
     P.kp = up(k, 16);
-    if (m <= FEW_ROWS) return P;
-    // the loads into LDS move 16 aligned bytes; rows whose length is no multiple of 16 need zeros behind them in one operand
+    if (few_rows(m, n, k, ((uintptr_t)w & 15) == 0 && (ld_w & 15) == 0)) return P;
+    // The loads into LDS move 16 aligned bytes; rows whose length is no multiple of 16 need zeros behind them in one operand: q's.
+    // (Of w the 16 aligned bytes that hold a row's last ones are read whole: never past what was allocated with them.)
     P.align_q = !q_padded && (((uintptr_t)q & 15) || (ld_q & 15) || (k & 15) || ld_q > TILE_MAX_LD);
     P.align_w = ((uintptr_t)w & 15) || (ld_w & 15) || ld_w > TILE_MAX_LD;
     P.q_bytes = P.align_q ? up256((size_t)m * P.kp) : 0;
     P.w_bytes = P.align_w ? up256((size_t)n * P.kp) : 0;
     auto tiles = [&](i64 e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
-    // a larger tile reads less per product, but must not be mostly padding and must fill the chip
+    // A larger tile reads less per product, but must not be mostly padding and must fill the chip: at least 200 of them (us; with
+    // 400 or 100 instead: 2048^3 17.2 | 22.8 with 400, 3000 x 3000 x 512 16.7 | 26.8 with 100).
     auto pays = [&](i64 e) { return tiles(e) >= 200 && tiles(e) * e * e <= tiles(e / 2) * (e / 2) * (e / 2) * 9 / 8; };
     P.tile = pays(256) ? 256 : pays(128) ? 128 : 64;
-    // k split over workgroups where the tiles are too few for the CUs, in parts of at least 16 steps (a join costs 5 us)
+    // k split over workgroups where the tiles are too few for the CUs, in parts of at least 16 steps (us, split | not:
+    // 65 x 64 x 8192 10.2 | 19.6, 128 x 128 x 4096 9.3 | 12.6, 256 x 256 x 2048 8.8 | 9.1)
     const u32 steps = (u32)((k + TILE_KB - 1) / TILE_KB);
     u32 splits = 1;
     if (P.tile == 64)
@@ -689,16 +702,15 @@ static void rows_go(const Rows& R, hipStream_t st) {
     const i64 b = (R.rows + 256 / LANES - 1) / (256 / LANES);
     k_i8_quantize<T, LANES, NP, FAST><<<dim3((u32)(b < 1 << 20 ? b : 1 << 20)), dim3(256), 0, st>>>(R);
 }
-// Few lanes to a row waste the fewest on its end and on its reduction (86016 rows of 144 pieces: 16 lanes 9 pieces 55 us,
-// 64 lanes 4 pieces 64 us, before the rest of the kernel was trimmed); with few rows it takes more lanes to fill the chip.
+// Few lanes to a row waste the fewest on its end and on its reduction; with few rows it takes more lanes to fill the chip (us, 16 lanes
+// | 64: 300 fp16 values, 16384 rows 8.1 | 10.0, 8192 rows 7.3 | 6.7; 1152 values, 65536 rows 41.3 | 42.8, 16384 rows 17.3 | 15.1).
 template <class T, bool FAST>
 static void rows_dispatch(const Rows& R, hipStream_t st) {
     const u32 P = R.pieces;
-    const bool many = R.rows >= 16384;
     if (P <= 4) rows_go<T, 4, 1, FAST>(R, st);
     else if (P <= 16) rows_go<T, 16, 1, FAST>(R, st);
-    else if (P <= 64 && many) rows_go<T, 16, 4, FAST>(R, st);
-    else if (P <= 144 && many) rows_go<T, 16, 9, FAST>(R, st);
+    else if (P <= 64 && R.rows >= 16384) rows_go<T, 16, 4, FAST>(R, st);
+    else if (P > 64 && P <= 144 && R.rows >= 32768) rows_go<T, 16, 9, FAST>(R, st);
     else if (P <= 64) rows_go<T, 64, 1, FAST>(R, st);
     else if (P <= 256) rows_go<T, 64, 4, FAST>(R, st);
     else if (P <= 512) rows_go<T, 256, 2, FAST>(R, st);

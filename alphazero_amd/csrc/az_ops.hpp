@@ -23,6 +23,9 @@ __device__ inline T from_f32(float v) {
     return (T)v;
 }
 
+// Loads above stay above (left alone, the compiler moves each one to its use to save registers, and every one waits for memory).
+__device__ inline void loads_first() { __builtin_amdgcn_sched_barrier(0); }
+
 inline size_t dtype_size(int dtype) { return dtype == AZ_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == AZ_F32 || dtype == AZ_F16 || dtype == AZ_BF16; }
 

@@ -51,9 +51,6 @@ __device__ inline int find_job(const Jobs& js, int block) {
     while (j + 1 < js.n && block >= js.first[j + 1]) j++;
     return j;
 }
-// Loads above stay above (left alone, the compiler moves each one to its use to save registers, and every one waits for memory).
-__device__ inline void loads_first() { __builtin_amdgcn_sched_barrier(0); }
-
 // what is orthogonalised, after k_ortho_norm has updated m: N values a thread, at `at` (where `in`; else zeros)
 template <class T, int N>
 __device__ inline void update_values(const Job& J, const Hyper& h, const i32 (&at)[N], const bool (&in)[N], float (&v)[N]) {
@@ -316,7 +313,7 @@ using OTile64 = TileShape<64, 64, 2, 2, 3, 4>;   // few tiles: what counts is th
 constexpr int NARROW = 128, NPANEL = 128, NTHREADS = 1024, NWAVES = 16;
 constexpr int NBUF = NARROW * 512;   // a row: 128 high halves, 128 low halves
 constexpr int NSTEP_LDS = 2 * NBUF + 32 * 1024;
-constexpr int MAX_GROUPS = 16;       // workgroups a matrix: each adds up that many partial Gram matrices
+constexpr int MAX_GROUPS = 64;       // workgroups a matrix: so many parts of the Gram matrix are added up
 
 __device__ inline int swap23(int i) { return (i & ~12) | ((i & 4) << 1) | ((i & 8) >> 1); }
 // byte of value k of a row; pieces of 16 bytes are exchanged by row & 15, so that 16 rows read at one k use all banks
@@ -451,13 +448,18 @@ __global__ __launch_bounds__(256) void k_narrow_sum(Jobs js) {
     const int blocks = nar_blocks(J), b = blockIdx.x, lane = threadIdx.x & 63, g4 = threadIdx.x >> 6;
     if (b >= blocks) return;
     const float* d = J.gram + ((i64)b * 64 + lane) * 16 + 4 * g4;
-    f32x4 y[MAX_GROUPS], sum = {0, 0, 0, 0};
+    constexpr int AHEAD = 16;
+    f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int g0 = 0; g0 < J.groups; g0 += AHEAD) {
+        f32x4 y[AHEAD];
 #pragma unroll
-    for (int g = 0; g < MAX_GROUPS; g++) y[g] = *(const f32x4*)(d + (i64)(g < J.groups ? g : 0) * blocks * 1024);
-    loads_first();
+        for (int g = 0; g < AHEAD; g++) y[g] = *(const f32x4*)(d + (i64)(g0 + g < J.groups ? g0 + g : 0) * blocks * 1024);
+        loads_first();
 #pragma unroll
-    for (int g = 0; g < MAX_GROUPS; g++)
-        if (g < J.groups) sum += y[g];
+        for (int g = 0; g < AHEAD; g++)
+            if (g0 + g < J.groups) sum += y[g];
+    }
     int bi, bj;
     lower_block(b, bi, bj);
     const int m = bi * 32 + acc_row(4 * g4, lane), n = bj * 32 + (lane & 31);
@@ -686,16 +688,18 @@ static int product_blocks(Jobs& js) {   // fills js.first
 }
 template <int MODE, class T>
 static void product(Jobs& js, const Hyper& h, int cur, hipStream_t st) {
-    // the larger tile reads half as much per product; it needs enough tiles to fill the chip
+    // The larger tile reads half as much per product; it needs enough tiles to fill the chip (us, from 80 tiles on | from 160 on:
+    // 1500 x 1500, 144 and 156 tiles, 392 | 512; 800 x 2000, 112 tiles, 248 | 241).
+    constexpr int ENOUGH = 120;
     if constexpr (MODE == GRAM || MODE == POLY) {
         const int n = product_blocks<MODE, OTile128s>(js);
-        if (n >= 160) {
+        if (n >= ENOUGH) {
             k_ortho_product<MODE, OTile128s, T><<<dim3((u32)n), dim3(OTile128s::THREADS), Staged<OTile128s>::LDS, st>>>(js, h, cur);
             return;
         }
     } else {
         const int n = product_blocks<MODE, OTile128>(js);
-        if (n >= 160) {
+        if (n >= ENOUGH) {
             k_ortho_product<MODE, OTile128, T><<<dim3((u32)n), dim3(OTile128::THREADS), Staged<OTile128>::LDS, st>>>(js, h, cur);
             return;
         }
