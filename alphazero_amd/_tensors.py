@@ -12,11 +12,11 @@ stream_of = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCu
 
 def same_device(what, first, *rest):
     """every tensor on one GPU; returns its ordinal.  There is no CPU path."""
-    if not first.is_cuda:
+    dev = first.get_device()   # -1: not on a device
+    if dev < 0 or not first.is_cuda:
         raise AzError("%s: tensors must be on the GPU (no CPU path)" % what)
-    dev = first.get_device()
     for t in rest:
-        if t is not None and not (t.is_cuda and t.get_device() == dev):
+        if t is not None and t.get_device() != dev:
             raise AzError("%s: tensors on different devices" % what)
     return dev
 
@@ -26,6 +26,11 @@ def no_grad(what, *tensors):
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise AzError("%s has no backward pass: call it under torch.no_grad() or detach its inputs" % what)
+
+
+def written(*tensors):
+    """tells autograd that a kernel wrote these in place: a backward pass that had saved one then says so"""
+    torch.autograd.graph.increment_version(tensors)
 
 
 def workspace(n, like):
@@ -39,9 +44,10 @@ def workspace(n, like):
 
 def rows_of(t, what, name):
     """a 2-D tensor whose rows are contiguous -> (rows, columns, distance between rows in elements)"""
-    if t.dim() != 2:
+    shape = t.shape
+    if len(shape) != 2:
         raise AzError("%s: %s must have two dimensions" % (what, name))
-    r, c = t.shape
+    r, c = shape
     if t.is_contiguous():
         return r, c, c
     ld, inner = t.stride()
@@ -56,6 +62,6 @@ def rows_of(t, what, name):
 
 def vector(t, n, what, name):
     """address of a contiguous float32 [n]"""
-    if t.dtype is not torch.float32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous():
         raise AzError("%s: %s must be a contiguous float32 [%d]" % (what, name, n))
     return t.data_ptr()

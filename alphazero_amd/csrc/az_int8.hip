@@ -725,9 +725,9 @@ static int rows_launch(Rows R, hipStream_t st) {
     R.pieces = (u32)(per * R.taps);
     R.magic = per > 1 && (u64)R.pieces * (u64)per < (u64)1 << 32 ? (u32)(((u64)1 << 32) / (u64)per + 1) : 0;
     R.inv_tap = 1.0f / (float)per;
-    const i64 row = R.ld_x * (i64)sizeof(T), bytes = R.n_src * row;
-    const bool fast = R.cols % Piece<T>::EPP == 0 && ((uintptr_t)R.x & 15) == 0 && row % 16 == 0 && row < 1 << 24 &&
-                      R.n_src < 1 << 24 && R.n_src > 0 && bytes < 0x7ffffff0;
+    const bool small = R.ld_x < 1 << 22 && R.n_src < 1 << 24 && R.n_src > 0;
+    const i64 row = small ? R.ld_x * (i64)sizeof(T) : 0;
+    const bool fast = small && R.cols % Piece<T>::EPP == 0 && ((uintptr_t)R.x & 15) == 0 && row % 16 == 0 && R.n_src * row < 0x7ffffff0;
     R.row_bytes = (u32)row;
     R.x_bytes = fast ? (u32)((R.n_src - 1) * row + R.cols * (i64)sizeof(T)) : 0;
     if (fast) rows_dispatch<T, true>(R, st);
@@ -766,7 +766,7 @@ int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const 
     if (!dtype_ok(dtype)) return refuse("az_i8_quantize: unknown dtype");
     if (rows < 0 || cols < 1 || n_src < 0 || ld_x < cols) return refuse("az_i8_quantize: bad shape or row distance");
     if (!index_dev && (taps != 1 || n_src != rows)) return refuse("az_i8_quantize: without an index taps is 1 and n_src is rows");
-    if (taps < 1 || cols > 0x7fffffff / taps || ld_q < taps * cols) return refuse("az_i8_quantize: bad taps or ld_q");
+    if (taps < 1 || cols > 0x7fffffff / taps || ld_x > (i64)1 << 40 || ld_q < taps * cols) return refuse("az_i8_quantize: bad taps or ld_q");
     if (rows == 0) {
         DeviceScope dev(device);
         return dev.rc;
@@ -780,7 +780,7 @@ int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const 
 static int mm_check(int64_t m, int64_t n, int64_t k, int64_t ld_x, int64_t ld_w, const void* res, int64_t ld_res, int act,
                     int dtype, int64_t ld_y) {
     if (!dtype_ok(dtype)) return refuse("az_i8_matmul: unknown dtype");
-    if (m < 0 || n < 0 || k < 1 || k > I8_MAX_K || m > (i64)1 << 40 || n > (i64)1 << 40)
+    if (m < 0 || n < 0 || k < 1 || k > I8_MAX_K || m > 0x7fffffff || n > 0x7fffffff)
         return refuse("az_i8_matmul: bad shape (k is 1..131071)");
     if (ld_x < k || ld_w < k || ld_y < n || (res && ld_res < n)) return refuse("az_i8_matmul: bad row distance");
     if (act < AZ_ACT_NONE || act > AZ_ACT_SILU) return refuse("az_i8_matmul: unknown activation");
@@ -788,7 +788,7 @@ static int mm_check(int64_t m, int64_t n, int64_t k, int64_t ld_x, int64_t ld_w,
 }
 
 size_t az_i8_matmul_ws(int64_t m, int64_t n, int64_t k, const int8_t* q_dev, int64_t ld_q, const int8_t* w_dev, int64_t ld_w) {
-    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K) return 0;
+    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K || m > 0x7fffffff || n > 0x7fffffff) return 0;
     return mm_plan(m, n, k, q_dev, ld_q, false, w_dev, ld_w).total();
 }
 
@@ -812,7 +812,7 @@ int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t* 
 static bool linear_fused(i64 m, i64 k) { return m <= LIN_ROWS && m * up(k, 64) <= LIN_LDS; }
 
 size_t az_i8_linear_ws(int64_t m, int64_t n, int64_t k, const int8_t* w_dev, int64_t ld_w) {
-    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K || linear_fused(m, k)) return 0;
+    if (m < 1 || n < 1 || k < 1 || k > I8_MAX_K || m > 0x7fffffff || n > 0x7fffffff || linear_fused(m, k)) return 0;
     return up256((size_t)m * linear_pitch(k)) + up256((size_t)m * 4) +
            mm_plan(m, n, k, nullptr, linear_pitch(k), true, w_dev, ld_w).total();
 }

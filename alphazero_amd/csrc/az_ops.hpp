@@ -41,8 +41,11 @@ inline bool dtype_ok(int dtype) { return dtype == AZ_F32 || dtype == AZ_F16 || d
 struct DeviceScope {
     int before = -1, rc = AZ_OK;
     explicit DeviceScope(int device) {
-        int n = 0;
-        if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) {
+        static const int n = [] {   // the number of devices does not change while the process lives
+            int k = 0;
+            return hipGetDeviceCount(&k) == hipSuccess ? k : 0;
+        }();
+        if (n <= 0) {
             (void)hipGetLastError();
             set_error("no usable HIP device: libazamd has no CPU path");
             rc = AZ_ERR_NO_DEVICE;

@@ -609,6 +609,9 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
 // ---------------------------------------------------------------------------------------------------- host side
 static i64 pad(i64 n) { return (n + OT - 1) / OT * OT; }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+}
 static bool dims_ok(i64 rows, i64 cols) { return rows >= 1 && cols >= 1 && rows <= ORTHO_MAX_DIM && cols <= ORTHO_MAX_DIM; }
 
 // lays a job's workspace out from `p` on (null: only counts) and returns its bytes
@@ -652,18 +655,19 @@ static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
     return off;
 }
 
-// Which coefficients keep the halves in range: follows the largest singular value through the steps on a fine grid.
+// Which coefficients keep the halves in range: follows the largest singular value through the steps on a grid.  (The limits below
+// leave a factor of two to where a high half would overflow: room for what lies between the grid's points.)
 static bool coeffs_ok(int steps, const double* k) {
     if (!k || !isfinite(k[0]) || !isfinite(k[1]) || !isfinite(k[2])) return false;
     double top = 1.0;
     for (int it = 0; it < steps; it++) {
         double next = 0;
-        for (int i = 0; i <= 4096; i++) {
-            const double x = top * i / 4096, x2 = x * x, poly = k[0] + k[1] * x2 + k[2] * x2 * x2;
+        for (int i = 0; i <= 256; i++) {
+            const double x = top * i / 256, x2 = x * x, poly = k[0] + k[1] * x2 + k[2] * x2 * x2;
             if (fabs(poly) > 15.9 || fabs(poly - k[0]) > 15.9) return false;
             next = fmax(next, fabs(poly * x));
         }
-        top = next * 1.001;
+        top = next * 1.01;
         if (top > 1.99) return false;
     }
     return true;
@@ -778,10 +782,13 @@ static int ortho_check(int dtype, int steps, const double* coeffs, double eps, c
 
 int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int64_t cols, const void* g_dev, void* out_dev,
                          int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes, void* stream) {
-    if (batch < 0 || !dims_ok(rows, cols)) return refuse("az_orthogonalize: bad shape (rows and cols are 1..32768)");
+    if (batch < 0 || batch > (i64)1 << 31 || !dims_ok(rows, cols))
+        return refuse("az_orthogonalize: bad shape (rows and cols are 1..32768)");
     int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_orthogonalize_ws(batch, rows, cols));
     if (rc != AZ_OK) return rc;
     if (batch > 0 && (!g_dev || !out_dev)) return refuse("az_orthogonalize: null pointer");
+    const size_t all = (size_t)batch * rows * cols * dtype_size(dtype);
+    if (g_dev != out_dev && overlap(g_dev, all, out_dev, all)) return refuse("az_orthogonalize: out overlaps g without being it");
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || batch == 0) return dev.rc;
     Hyper h = {};
@@ -832,9 +839,6 @@ int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n
         if (!items[i].w_dev || !items[i].g_dev || !items[i].m_dev) return refuse("az_muon_step: null pointer");
     }
     // what is written (w, m) overlaps nothing else
-    auto overlap = [](const void* p, size_t np, const void* q, size_t nq) {
-        return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
-    };
     for (int64_t i = 0; i < n; i++) {
         const size_t ni = (size_t)items[i].rows * items[i].cols, es = dtype_size(dtype);
         for (int64_t k = 0; k < n; k++) {

@@ -6,7 +6,7 @@ import torch
 
 from . import _abi
 from ._abi import AzError, check, lib
-from ._tensors import DTYPES, no_grad, rows_of, same_device, stream_of, vector, workspace
+from ._tensors import DTYPES, no_grad, rows_of, same_device, stream_of, vector, workspace, written
 
 MAX_K = 131071   # the longest sum of products of two 8-bit integers that int32 holds
 
@@ -62,6 +62,7 @@ def _layer(what, m, k, w, w_scale, bias, residual, act, dtype, out):
     if out is None:
         out, ld_y = torch.empty((m, n), dtype=dtype, device=w.device), n
     else:
+        written(out)
         o_m, o_n, ld_y = rows_of(out, what, "out")
         if out.dtype is not dtype or o_m != m or o_n != n:
             raise AzError("%s: out must be [%d, %d] of the output's dtype" % (what, m, n))

@@ -7,7 +7,7 @@ import torch
 
 from . import _abi
 from ._abi import AzError, check, lib
-from ._tensors import DTYPES, no_grad, same_device, stream_of, workspace
+from ._tensors import DTYPES, no_grad, same_device, stream_of, workspace, written
 
 COEFFS = (3.4445, -4.7750, 2.0315)
 
@@ -39,6 +39,7 @@ def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, out=None):
     ws, wsp = workspace(nws, g)
     check(L.az_orthogonalize_dev(dev, DTYPES[g.dtype], batch, rows, cols, g.data_ptr(), out.data_ptr(), steps, _coeffs(coeffs),
                                  eps, wsp, nws, stream_of(dev)))
+    written(out)
     return out
 
 
@@ -77,6 +78,7 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
     ws, wsp = workspace(nws, weights[0])
     check(L.az_muon_step_dev(dev, DTYPES[dt], items, n, lr, momentum, 1 if nesterov else 0, weight_decay, steps, _coeffs(coeffs),
                              eps, wsp, nws, stream_of(dev)))
+    written(*weights, *momenta)
 
 
 class Muon(torch.optim.Optimizer):

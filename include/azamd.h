@@ -293,6 +293,7 @@ int az_net_forward_dev(az_engine *e, int64_t n, const uint64_t *states_dev, floa
  * between az_select and az_backup; its weights are trained outside).  Pointers ending in _dev are memory of `device`;
  * every call is asynchronous on `stream` (a hipStream_t of that device; NULL = its default stream), allocates nothing,
  * keeps nothing and may be captured into a HIP graph.  Calls may overlap in time if their outputs and workspaces do not.
+ * Outputs must not overlap inputs but where a call says so.
  * `ws_dev`: workspace of at least the bytes that the matching *_ws function returns, aligned to 256 bytes, contents
  * irrelevant before and after; less than that is AZ_ERR_ARG.  The caller's current device is restored. */
 #define AZ_F32 0
@@ -329,7 +330,7 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void *x_
 
 /* Orthogonalisation of `batch` matrices [rows][cols] (contiguous) by Newton-Schulz products: X = G / (||G||_F + eps), then
  * `steps` times X <- a X + (b A + c A^2) X with A = X X^T (on the shorter side), coeffs = {a, b, c}.  Products are
- * float32-accurate (fp16 matrix pipe, operands split into two halves); out may be g.  steps 1..16, eps > 0.  Coefficients whose
+ * float32-accurate (fp16 matrix pipe, operands split into two halves); out may be g itself.  steps 1..16, eps > 0.  Coefficients whose
  * iteration takes a singular value of [0, 1] above 2, or b A + c A^2 + a out of [-16, 16], are AZ_ERR_ARG (the halves' range).
  * A matrix that holds a NaN or an infinity comes out as NaN.  rows, cols <= 32768. */
 size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols);

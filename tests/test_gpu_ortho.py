@@ -215,3 +215,24 @@ def test_refusals(O):
             call()
     assert (x == 1).all() and (m == 0).all()
     O.muon_step([], [], [], lr=0.1)
+    z = torch.randn(100).cuda()
+    with pytest.raises(AzError):
+        O.orthogonalize(z[:48].view(6, 8), out=z[8:56].view(6, 8))
+
+
+def test_in_place_updates_are_seen_by_autograd(O):
+    """a weight that a graph has saved and that is updated before its backward pass: an error, not a wrong gradient"""
+    w = torch.nn.Parameter(torch.randn(6, 8).cuda())
+    x = torch.randn(8, 3, requires_grad=True, device="cuda")
+    y = (w @ x).sum()
+    O.muon_step([w.detach()], [torch.ones(6, 8).cuda()], [torch.zeros(6, 8).cuda()], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_repeated_calls_give_the_same_bits(O):
+    for shape in ((3, 128, 1152), (1, 300, 700), (2, 640, 640), (1, 1500, 1500)):
+        g = torch.randn(shape).cuda()
+        first = O.orthogonalize(g)
+        for _ in range(3):
+            assert torch.equal(O.orthogonalize(g), first)
