@@ -387,7 +387,28 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
         const bool two = W == 2 && n + 1 < p.n;
         if (n >= p.n) continue;
 #pragma unroll
-        for (int i = 0; i < S::FM; i++)
+        for (int i = 0; i < S::FM; i++) {
+            float res[16][W];
+            if (p.res && !part) {   // a block's residuals on their way at once
+                T raw[16][W];
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const i64 m = m0 + wm + 32 * i + acc_row(r, lane);
+                    const T* s = (const T*)p.res + (m < p.m ? m : p.m - 1) * p.ld_res + n;
+                    raw[r][0] = s[0];
+                    if (W == 2) raw[r][W - 1] = s[two ? 1 : 0];
+                }
+                loads_first();
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+#pragma unroll
+                    for (int k = 0; k < W; k++) res[r][k] = to_f32(raw[r][k]);
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+#pragma unroll
+                    for (int k = 0; k < W; k++) res[r][k] = -0.0f;   // adds nothing, not even a sign
+            }
 #pragma unroll
             for (int g = 0; g < 4; g++) {
                 const int row = wm + 32 * i + acc_row(4 * g, lane);
@@ -402,13 +423,8 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
                         if (two) part[m * p.n + n + 1] = q1;
                         continue;
                     }
-                    float v0 = (float)q0 * s4[e] * s0 + b0, v1 = (float)q1 * s4[e] * s1 + b1;
+                    float v0 = (float)q0 * s4[e] * s0 + b0 + res[4 * g + e][0], v1 = (float)q1 * s4[e] * s1 + b1 + res[4 * g + e][W - 1];
                     T* y = (T*)p.y + m * p.ld_y + n;
-                    if (p.res) {
-                        const T* r = (const T*)p.res + m * p.ld_res + n;
-                        v0 += to_f32(r[0]);
-                        if (two) v1 += to_f32(r[1]);
-                    }
                     v0 = activate<T>(v0, p.act);
                     if (two && p.pair_store) {
                         struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
@@ -419,6 +435,7 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
                     }
                 }
             }
+        }
     }
 }
 template <class T>
