@@ -29,7 +29,7 @@ struct Job {
     i32 rows, cols, s, l, sp, lp, n_part;
     float kappa;
     double* part;
-    u8 *x, *t0, *t1, *a, *b;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
+    u8 *x, *t0, *t1, *a, *b, *c, *d;   // split operands in panels: 16 values of every row (16 hi, 16 lo: 64 bytes), then the next 16
     // short side <= 128 (see "Narrow matrices"): T in MFMA order in t, partial Gram matrices in gram
     float* gram;
     u8* image;
@@ -173,14 +173,30 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     }
 }
 
-enum { GRAM = 0, POLY = 1, STEP = 2, LAST = 3 };
-// GRAM: A = X X^T     POLY: B = a I + b A + c A A^T     STEP: T <- T B (and X)     LAST: the output, in its own orientation
-// A and B are symmetric: their launches compute the tiles that touch the lower triangle and store them twice.
+enum { GRAM = 0, POLY = 1, SQUARE = 2, STEP = 3, LAST = 4 };
+// GRAM: A = X X^T     POLY: B = a I + b A + c A A^T     SQUARE: a product of two of the s x s matrices     STEP: T <- T B (and X)
+// LAST: the output, in its own orientation.
+// The s x s matrices are polynomials of A: symmetric, and they commute.  Their launches compute the tiles that touch the lower
+// triangle and store them twice.
+//
+// Several steps at once.  A step on X costs 2.4 s^2 l multiplications and 0.8 s^3 (a symmetric product takes 0.8 of a whole one's
+// time).  Two or three can be made on the s x s side alone, A <- B A B and P <- B P, with X <- P X at their end: the default's five
+// steps cost 3.6 s^2 l + 11.2 s^3 as 2 + 3 against 9 s^2 l + 4 s^3 one by one, less from l = 1.33 s on.  All five at once would
+// not do: P's coefficients grow by (a^2)^k, and with them A's rounding; after two steps on X the small singular values have
+// grown by a^2 = 12 and 2 + 3 is as accurate as step by step (float32: 1.3e-6 to 4.1e-6 against 1.3e-6, 4.6e-5 for all five).
+
+// what a launch multiplies: s x s matrices 0..3 (a, b, c, d), and the power of two from its sums to what it stores
+struct Op {
+    int p, q, out;
+    float unit;
+};
+__device__ inline u8* square(const Job& J, int i) { return i == 0 ? J.a : i == 1 ? J.b : i == 2 ? J.c : J.d; }
+__host__ __device__ constexpr bool symmetric(int mode) { return mode == GRAM || mode == POLY || mode == SQUARE; }
 
 // rows and columns of a launch's result (padded)
 __host__ __device__ inline void product_dims(int mode, const Job& J, int& rows, int& cols) {
     const bool flip = J.rows > J.cols;
-    rows = mode == GRAM || mode == POLY ? J.sp : (mode == STEP || flip ? J.lp : J.sp);
+    rows = symmetric(mode) ? J.sp : (mode == STEP || flip ? J.lp : J.sp);
     cols = mode == LAST && !flip ? J.lp : J.sp;
 }
 // the tile's result passes through LDS as float32, so that rows leave it 16 bytes a lane
@@ -192,20 +208,21 @@ struct Staged {
 };
 
 template <int MODE, class S, class T>
-__global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur) {
+__global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur, Op op) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     const int ji = find_job(js, blockIdx.x), tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Job J = js.j[ji];
     const bool flip = J.rows > J.cols;
-    constexpr bool SYM = MODE == GRAM || MODE == POLY;
+    constexpr bool SYM = symmetric(MODE);
     u8 *const t_cur = cur ? J.t1 : J.t0, *const t_next = cur ? J.t0 : J.t1;
     const u8 *P, *Q;
     int kp, rows, cols;
     product_dims(MODE, J, rows, cols);
     if (MODE == GRAM) { P = Q = J.x; kp = J.lp; }
     else if (MODE == POLY) { P = Q = J.a; kp = J.sp; }
-    else if (MODE == STEP || flip) { P = t_cur; Q = J.b; kp = J.sp; }
-    else { P = J.b; Q = t_cur; kp = J.sp; }
+    else if (MODE == SQUARE) { P = square(J, op.p); Q = square(J, op.q); kp = J.sp; }
+    else if (MODE == STEP || flip) { P = t_cur; Q = square(J, op.q); kp = J.sp; }
+    else { P = square(J, op.q); Q = t_cur; kp = J.sp; }
     u32 tm, tn;
     const int block = blockIdx.x - js.first[ji];
     if (SYM) symmetric_place(block, (rows + S::BM - 1) / S::BM, S::BM / S::BN, (cols + S::BN - 1) / S::BN, tm, tn);
@@ -218,7 +235,6 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
     tile_product<KindSplit, S>(KindSplit(), p, q, 0, kp * 4, lds, wave, lane, acc);
 
     constexpr int W = S::PAIRS ? 2 : 1, PITCH = Staged<S>::PITCH;
-    constexpr float UNIT = MODE == GRAM ? 0x1p-16f : MODE == POLY ? 0x1p-24f : MODE == STEP ? 0x1p-11f : 0x1p-25f;
     float* tile = (float*)lds;
 #pragma unroll
     for (int i = 0; i < S::FM; i++)
@@ -228,12 +244,12 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
             for (int r = 0; r < 16; r++) {
                 float* d = tile + (wave / S::WN * (S::FM * 32) + 32 * i + acc_row(r, lane)) * PITCH + wave % S::WN * (S::FN * 32) +
                            32 * j + W * (lane & 31);
-                d[0] = acc[i][j][r] * UNIT;
-                if (W == 2) d[1] = acc[i][j + W - 1][r] * UNIT;
+                d[0] = acc[i][j][r] * op.unit;
+                if (W == 2) d[1] = acc[i][j + W - 1][r] * op.unit;
             }
     __syncthreads();
     if (MODE != LAST) {   // mrows and ncols are multiples of 64 here
-        u8* out = MODE == GRAM ? J.a : MODE == POLY ? J.b : t_next;
+        u8* out = MODE == GRAM ? J.a : SYM ? square(J, op.out) : t_next;
         // 32 lanes store 16 values of 16 rows, 1 KB in a run: 16 lanes the first eight, 16 the others (16 rows read from LDS at
         // one column are on different banks)
 #pragma unroll 2
@@ -641,7 +657,7 @@ static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
         J.t1 = take((size_t)panels * NPANEL * NARROW * 4);
         J.gram = (float*)take((size_t)J.groups * (J.nb * (J.nb + 1) / 2) * 4096);
         J.image = take(NBUF);
-        J.x = J.a = J.b = nullptr;
+        J.x = J.a = J.b = J.c = J.d = nullptr;
         return off;
     }
     J.gram = nullptr;
@@ -652,6 +668,8 @@ static size_t plan(Job& J, i64 rows, i64 cols, char* p) {
     J.t1 = take((size_t)J.sp * J.lp * 4);
     J.a = take((size_t)J.sp * J.sp * 4);
     J.b = take((size_t)J.sp * J.sp * 4);
+    J.c = take((size_t)J.sp * J.sp * 4);
+    J.d = take((size_t)J.sp * J.sp * 4);
     return off;
 }
 
@@ -673,6 +691,43 @@ static bool coeffs_ok(int steps, const double* k) {
     return true;
 }
 
+static double step_poly(const Hyper& h, double x2) { return h.a + h.b * x2 + h.c * x2 * x2; }
+// the largest singular value after a step, from the largest before it
+static double top_after(const Hyper& h, double top) {
+    double next = 0;
+    for (int i = 0; i <= 256; i++) next = fmax(next, fabs(step_poly(h, top * i / 256 * (top * i / 256)) * top * i / 256));
+    return next * 1.01;
+}
+
+// how much a step A <- B A B can enlarge an error of A: the largest slope of y p(y)^2 (a^2 = 12 for the default coefficients)
+static double steepest(const Hyper& h, int steps) {
+    double top = 1.0, most = 0;
+    for (int it = 0; it < steps; it++, top = top_after(h, top))
+        for (int i = 0; i <= 256; i++) {
+            const double y = top * top * i / 256, p = step_poly(h, y);
+            most = fmax(most, fabs(p * p + 2 * y * p * (h.b + 2 * h.c * y)));
+        }
+    return most;
+}
+
+// the power of two that keeps the product of `n` steps' B, from step `first` on, inside fp16's range
+static int product_exponent(const Hyper& h, int first, int n) {
+    double top = 1.0, most = 1.0;
+    for (int it = 0; it < first; it++) top = top_after(h, top);
+    for (int i = 0; i <= 256; i++) {
+        double x = top * i / 256, product = 1.0;
+        for (int k = 0; k < n; k++) {
+            const double p = step_poly(h, x * x);
+            product *= p;
+            x *= p;
+            most = fmax(most, fabs(product));
+        }
+    }
+    int e = 11;
+    while (ldexp(most, e) > 32000.0) e--;   // a factor of two for what lies between the grid's points
+    return e;
+}
+
 template <class F>
 static void each_first(Jobs& js, F blocks) {
     js.first[0] = 0;
@@ -684,32 +739,32 @@ static int product_blocks(Jobs& js) {   // fills js.first
     each_first(js, [](const Job& J) {
         int rows, cols;
         product_dims(MODE, J, rows, cols);
-        if (MODE == GRAM || MODE == POLY)
+        if (symmetric(MODE))
             return (i64)symmetric_total((rows + S::BM - 1) / S::BM, S::BM / S::BN, (cols + S::BN - 1) / S::BN);
         return (i64)((rows + S::BM - 1) / S::BM) * ((cols + S::BN - 1) / S::BN);
     });
     return js.first[js.n];
 }
 template <int MODE, class T>
-static void product(Jobs& js, const Hyper& h, int cur, hipStream_t st) {
+static void product(Jobs& js, const Hyper& h, int cur, const Op& op, hipStream_t st) {
     // The larger tile reads half as much per product; it needs enough tiles to fill the chip (us, from 80 tiles on | from 160 on:
     // 1500 x 1500, 144 and 156 tiles, 392 | 512; 800 x 2000, 112 tiles, 248 | 241).
     constexpr int ENOUGH = 120;
-    if constexpr (MODE == GRAM || MODE == POLY) {
+    if constexpr (symmetric(MODE)) {
         const int n = product_blocks<MODE, OTile128s>(js);
         if (n >= ENOUGH) {
-            k_ortho_product<MODE, OTile128s, T><<<dim3((u32)n), dim3(OTile128s::THREADS), Staged<OTile128s>::LDS, st>>>(js, h, cur);
+            k_ortho_product<MODE, OTile128s, T><<<dim3((u32)n), dim3(OTile128s::THREADS), Staged<OTile128s>::LDS, st>>>(js, h, cur, op);
             return;
         }
     } else {
         const int n = product_blocks<MODE, OTile128>(js);
         if (n >= ENOUGH) {
-            k_ortho_product<MODE, OTile128, T><<<dim3((u32)n), dim3(OTile128::THREADS), Staged<OTile128>::LDS, st>>>(js, h, cur);
+            k_ortho_product<MODE, OTile128, T><<<dim3((u32)n), dim3(OTile128::THREADS), Staged<OTile128>::LDS, st>>>(js, h, cur, op);
             return;
         }
     }
     const int n = product_blocks<MODE, OTile64>(js);
-    k_ortho_product<MODE, OTile64, T><<<dim3((u32)n), dim3(OTile64::THREADS), Staged<OTile64>::LDS, st>>>(js, h, cur);
+    k_ortho_product<MODE, OTile64, T><<<dim3((u32)n), dim3(OTile64::THREADS), Staged<OTile64>::LDS, st>>>(js, h, cur, op);
 }
 
 static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_t st) {
@@ -744,16 +799,52 @@ static int run_jobs(Jobs& all, const Hyper& h, int steps, int dtype, hipStream_t
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
-    int cur = 0;
-    for (int it = 0; it < steps; it++) {
-        product<GRAM, float>(js, h, cur, st);
-        product<POLY, float>(js, h, cur, st);
-        if (it + 1 < steps) {
-            product<STEP, float>(js, h, cur, st);
+    // steps on the s x s side where that is less work in all
+    int len[16], n = 0, left = steps;
+    double one_by_one = 0, several = 0;
+    while (left > 0) {
+        len[n] = n == 0 ? (left < 2 ? left : 2) : (left < 3 ? left : 3);
+        left -= len[n++];
+    }
+    for (int i = 0; i < js.n; i++) {
+        const double s = js.j[i].sp, l = js.j[i].lp;
+        one_by_one += steps * (1.8 * s * s * l + 0.8 * s * s * s);
+        for (int k = 0; k < n; k++) several += 1.8 * s * s * l + 0.8 * s * s * s * (len[k] == 1 ? 1 : len[k] == 2 ? 5 : 9);
+    }
+    // 2 + 3 is 18 launches against 15.  Measured, 2 + 3 | one by one: 1024 x 1536 251 | 247 us (0.95 of the work), 2 x 400 x 800
+    // 158 | 147 and 1024 x 2048 264 | 273 (0.84), 300 x 2000 151 | 167 (0.57), 1024 x 4096 309 | 377 (0.64)
+    if (several > 0.8 * one_by_one || steepest(h, steps) > 16.0)
+        for (n = 0; n < steps; n++) len[n] = 1;
+    const Op gram = {0, 0, 0, 0x1p-16f};                                  // 2^14 2^14 -> 2^12
+    auto poly = [](int out) { return Op{0, 0, out, 0x1p-24f}; };           // 2^12 2^12 -> 1, then 2^11
+    auto to_a = [](int p, int q, int out) { return Op{p, q, out, 0x1p-11f}; };   // 2^11 2^12 -> 2^12
+    int cur = 0, done = 0;
+    for (int k = 0; k < n; k++) {
+        product<GRAM, float>(js, h, cur, gram, st);
+        product<POLY, float>(js, h, cur, poly(1), st);
+        int by = 1, e = 11;   // X is multiplied by matrix `by`, kept times 2^e
+        if (len[k] > 1) {
+            e = product_exponent(h, done, len[k]);
+            product<SQUARE, float>(js, h, cur, to_a(1, 0, 2), st);          // c = B A
+            product<SQUARE, float>(js, h, cur, to_a(2, 1, 0), st);          // a = B A B: the next step's A
+            product<POLY, float>(js, h, cur, poly(3), st);                  // d: the next step's B
+            product<SQUARE, float>(js, h, cur, Op{3, 1, 2, ldexpf(1.0f, e - 22)}, st);   // c = P of two steps
+            by = 2;
+        }
+        if (len[k] > 2) {
+            product<SQUARE, float>(js, h, cur, to_a(3, 0, 1), st);
+            product<SQUARE, float>(js, h, cur, to_a(1, 3, 0), st);
+            product<POLY, float>(js, h, cur, poly(3), st);
+            product<SQUARE, float>(js, h, cur, Op{3, 2, 1, 0x1p-11f}, st);  // b = P of three: 2^11 2^e -> 2^e
+            by = 1;
+        }
+        if (k + 1 < n) {
+            product<STEP, float>(js, h, cur, Op{0, by, 0, ldexpf(1.0f, -e)}, st);
         } else {
-            AZ_DISPATCH_DTYPE(dtype, product<LAST, T>(js, h, cur, st));
+            AZ_DISPATCH_DTYPE(dtype, product<LAST, T>(js, h, cur, Op{0, by, 0, ldexpf(1.0f, -14 - e)}, st));
         }
         cur ^= 1;
+        done += len[k];
     }
     return launch_status("az_orthogonalize");
 }

@@ -49,7 +49,8 @@ def gradient(rows, cols, seed, scale=1e-3):
 
 
 SHAPES = [(1, 1), (1, 7), (7, 1), (3, 5), (16, 16), (27, 128), (128, 27), (64, 64), (65, 63), (128, 128), (128, 1152), (129, 40),
-          (1152, 128), (130, 131), (200, 333), (333, 200), (255, 1000), (1, 3000), (100, 5000), (384, 384), (640, 513)]
+          (1152, 128), (130, 131), (200, 333), (333, 200), (255, 1000), (1, 3000), (100, 5000), (384, 384), (640, 513),
+          (130, 2000), (1100, 300), (256, 512)]
 
 
 @pytest.mark.parametrize("dt", list(DT))
@@ -62,13 +63,25 @@ def test_orthogonalize(O, rows, cols, dt):
     assert float((y.cpu().double() - want).norm()) <= tol
 
 
-@pytest.mark.parametrize("rows,cols", [(40, 70), (70, 40), (200, 300)])
+@pytest.mark.parametrize("rows,cols", [(40, 70), (70, 40), (200, 300), (150, 900)])
 @pytest.mark.parametrize("kw", [dict(steps=1), dict(steps=2, coeffs=(1.5, -0.5, 0.0)), dict(steps=12, coeffs=(1.5, -0.5, 0.0)),
                                 dict(steps=16), dict(steps=3, eps=1e-3), dict(steps=3, coeffs=(2.0, -1.5, 0.5))])
 def test_steps_and_coefficients(O, rows, cols, kw):
     g = gradient(rows, cols, 3)
     want, tol = allowed(g, torch.float32, **kw)
     assert float((O.orthogonalize(g.cuda(), **kw).cpu().double() - want).norm()) <= tol
+
+
+@pytest.mark.parametrize("noise", [0.5, 1e-3, 0.0])
+@pytest.mark.parametrize("steps", [2, 3, 4, 6, 8])
+def test_wide_matrices_of_low_rank(O, steps, noise):
+    """the steps taken on the short side's products alone, down to singular values of nothing"""
+    gen = torch.Generator().manual_seed(steps)
+    g = torch.randn(160, 6, generator=gen) @ torch.randn(6, 1500, generator=gen) + noise * torch.randn(160, 1500, generator=gen)
+    for m in (g, g.t().contiguous()):
+        y = O.orthogonalize(m.cuda(), steps=steps)
+        want, tol = allowed(m, torch.float32, steps=steps)
+        assert float((y.cpu().double() - want).norm()) <= tol
 
 
 def test_cubic_iteration_converges_to_the_polar_factor(O):
