@@ -164,7 +164,9 @@ __device__ inline u32 lanes_max(u32 v) {
 // LANES lanes to a row, NP pieces of 16 bytes to a lane: the row is read once and stays in registers between its largest
 // magnitude and its integers.  FAST: the columns are whole pieces, rows are 16-byte aligned, offsets fit 31 bits and the factors
 // of a row's offset 24 (full-rate multiplications); rows that are not there are read behind the end of the buffer, as zeros.
-// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 43 us, 2.9 TB/s; the VALU is busy for two thirds of it.
+// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 43 us, 2.8 TB/s of the 5.1 that a copy reaches; the VALU is busy for two
+// thirds of it (the exact quotient, its tie, the packing).  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
+// One row of 4096 bf16: 3.6 us, all of it latency: the load, the reduction over 4 waves, the launch.
 template <class T, int LANES, int NP, bool FAST>
 __global__ __launch_bounds__(256) void k_i8_quantize(Rows R) {
     constexpr int PER_BLOCK = 256 / LANES, EPP = Piece<T>::EPP;
@@ -258,7 +260,7 @@ __global__ __launch_bounds__(256) void k_i8_quantize(Rows R) {
         }
     }
 }
-// rows of more than 256 * 8 pieces: a workgroup a row, read twice
+// rows of more than 256 * 8 pieces: a workgroup a row, read twice (the second time from L2, as a row is 32 KB and more)
 template <class T>
 __global__ __launch_bounds__(256) void k_i8_quantize_long(Rows R) {
     __shared__ u32 part[4];
@@ -349,6 +351,10 @@ __device__ inline void put(const Mm& p, i64 m, i64 n, int sum, float scale) {
 
 // Rows of both operands at multiples of 16 bytes, k a multiple of 16.  blockIdx.y: which of the `splits` parts of k (whole
 // steps each); with more than one the int32 sums go to part[split][m][n] and k_i8_join adds them.
+// 8192^3, 256 x 256 tiles: 532-576 us, 1.9-2.1 POP/s of the 2.5 that the library's product reaches; the matrix pipe is busy for 59 % at
+// 1.66 GHz (power): a k slice costs as many LDS cycles as MFMA cycles.  86016 x 128 x 1152, 128 x 128 tiles: 33 us, 3.7 TB/s of the
+// rows it has to read, with SiLU and fp16 stores.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 9.2 us, one after the other:
+// launch, first tiles, 17 steps, scales and residual, stores.
 template <class T, class S>
 __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u32 tiles_n, u32 steps_per_split, int* part) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
@@ -438,6 +444,7 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
         }
     }
 }
+// the parts' sums, and the product's epilogue: 128 x 128 x 4096 in 8 parts, with the tiles, 9.3 us
 template <class T>
 __global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __restrict__ part) {
     const i64 total = p.m * p.n;
@@ -450,7 +457,8 @@ __global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __
 
 // Few rows (m <= 16 FM): a workgroup's 8 waves share 16 channels and split k between them, 64 bytes of a row a step, and add
 // their int32 sums in LDS.  What bounds it is reading w once: each wave asks for its share of 16 rows, 64 contiguous bytes of
-// a row per 4 lanes, with nothing between the loads.  Any alignment.
+// a row per 4 lanes, with nothing between the loads.  Any alignment.  1 x 4096 x 4096: 5.0 us, 3.4 TB/s of w; 42 x 128 x 1152: 4.6 us
+// on 8 workgroups, latency.
 constexpr int FEW_WAVES = 8;
 template <class T, int FM>
 __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_mm_few(Mm p) {
@@ -583,7 +591,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T*
 }
 
 // Rows of k bytes at any address -> rows of kp (a multiple of 16) with zeros behind k.  16 output bytes a thread; blockIdx.y: which
-// operand.
+// operand.  (777 + 1003) x 1031: 4.4 us, a launch and one trip to memory.
 struct Align {
     const i8* src[2];
     i64 ld[2], rows[2];
@@ -616,9 +624,9 @@ static bool few_rows(i64 m, i64 n, i64 k, bool aligned) {
 }
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
-using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;
+using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;   // 128 KB; 128 x 64 a wave: 6 operand reads for 8 MFMAs
 using Tile128 = TileShape<128, 128, 4, 2, 3, 1>;   // 48 KB: three workgroups a CU, whose stores run under each other's loads
-using Tile64 = TileShape<64, 64, 2, 2, 3, 2>;
+using Tile64 = TileShape<64, 64, 2, 2, 3, 2>;      // few tiles: what counts is the way from step to step, so a barrier every two
 
 // How a product is computed; a function of the sizes and alignments alone, so that the workspace can be asked for first.
 struct MmPlan {
