@@ -797,6 +797,11 @@ int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const 
         return dev.rc;
     }
     if ((!x_dev && n_src > 0) || !q_dev || !scale_dev) return refuse("az_i8_quantize: null pointer");
+    const i64 es = (i64)dtype_size(dtype);
+    const Span x = {x_dev, n_src, cols * es, ld_x * es}, q = {q_dev, rows, (i64)taps * cols, ld_q}, s = {scale_dev, 1, rows * 4, rows * 4};
+    const Span at = {index_dev, 1, rows * taps * 4, rows * taps * 4};
+    if (overlap(q, x) || overlap(q, s) || overlap(x, s) || overlap(q, at) || overlap(s, at))
+        return refuse("az_i8_quantize: q and scale must not overlap an input or each other");
     DeviceScope dev(device);
     if (dev.rc != AZ_OK) return dev.rc;
     return i8_quantize(dtype, rows, cols, x_dev, ld_x, n_src, index_dev, taps, q_dev, ld_q, false, scale_dev, (hipStream_t)stream);
@@ -809,6 +814,20 @@ static int mm_check(int64_t m, int64_t n, int64_t k, int64_t ld_x, int64_t ld_w,
         return refuse("az_i8_matmul: bad shape (k is 1..131071)");
     if (ld_x < k || ld_w < k || ld_y < n || (res && ld_res < n)) return refuse("az_i8_matmul: bad row distance");
     if (act < AZ_ACT_NONE || act > AZ_ACT_SILU) return refuse("az_i8_matmul: unknown activation");
+    return AZ_OK;
+}
+
+// y may be the residual itself (each element is read by the thread that writes it, before that); nothing else may be written
+static int y_check(const void* y, i64 m, i64 n, i64 ld_y, int dtype, const Span& x, const float* x_scale, const i8* w, i64 k, i64 ld_w,
+                   const float* w_scale, const float* bias, const void* res, i64 ld_res) {
+    const i64 es = (i64)dtype_size(dtype);
+    const Span out = {y, m, n * es, ld_y * es};
+    const Span in[] = {x, {x_scale, 1, m * 4, m * 4}, {w, n, k, ld_w}, {w_scale, 1, n * 4, n * 4}, {bias, 1, n * 4, n * 4}};
+    for (const Span& s : in)
+        if (overlap(out, s)) return refuse("az_i8_matmul: the output must not overlap an input");
+    const bool itself = res == y && (ld_res == ld_y || m == 1);
+    if (!itself && overlap(out, Span{res, m, n * es, ld_res * es}))
+        return refuse("az_i8_matmul: the output must be the residual or not overlap it");
     return AZ_OK;
 }
 
@@ -828,6 +847,9 @@ int az_i8_matmul_dev(int device, int64_t m, int64_t n, int64_t k, const int8_t* 
         return refuse("az_i8_matmul: workspace too small or not aligned to 256 bytes");
     if (m > 0 && n > 0 && (!q_dev || !q_scale_dev || !w_dev || !w_scale_dev || !y_dev))
         return refuse("az_i8_matmul: null pointer");
+    const int ok = y_check(y_dev, m, n, ld_y, dtype, Span{q_dev, m, k, ld_q}, q_scale_dev, w_dev, k, ld_w, w_scale_dev, bias_dev,
+                           residual_dev, ld_res);
+    if (ok != AZ_OK) return ok;
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || m == 0 || n == 0) return dev.rc;
     const Mm p = {m, n, k, q_dev, w_dev, ld_q, ld_w, q_scale_dev, w_scale_dev, bias_dev, residual_dev, ld_res, y_dev, ld_y, act, pairs_ok(y_dev, ld_y, dtype)};
@@ -852,6 +874,10 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void* x_
     if (ws_bytes < need || (need && (!ws_dev || ((uintptr_t)ws_dev & 255))))
         return refuse("az_i8_linear: workspace too small or not aligned to 256 bytes");
     if (m > 0 && n > 0 && (!x_dev || !w_dev || !w_scale_dev || !y_dev)) return refuse("az_i8_linear: null pointer");
+    const i64 es = (i64)dtype_size(dtype);
+    rc = y_check(y_dev, m, n, ld_y, dtype, Span{x_dev, m, k * es, ld_x * es}, nullptr, w_dev, k, ld_w, w_scale_dev, bias_dev, residual_dev,
+                 ld_res);
+    if (rc != AZ_OK) return rc;
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || m == 0 || n == 0) return dev.rc;
     hipStream_t st = (hipStream_t)stream;

@@ -13,6 +13,10 @@
 // then read both operands along their rows:  A = X X^T,  A^2 = A A^T,  T <- T B  (A and B are symmetric).
 #include <math.h>
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "az_tile.hpp"
 
 namespace az {
@@ -633,9 +637,6 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
 // ---------------------------------------------------------------------------------------------------- host side
 static i64 pad(i64 n) { return (n + OT - 1) / OT * OT; }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
-    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
-}
 static bool dims_ok(i64 rows, i64 cols) { return rows >= 1 && cols >= 1 && rows <= ORTHO_MAX_DIM && cols <= ORTHO_MAX_DIM; }
 
 // lays a job's workspace out from `p` on (null: only counts) and returns its bytes
@@ -913,6 +914,28 @@ int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int
     return AZ_OK;
 }
 
+// what is written (w, m) overlaps nothing else: all of them in the order of their addresses, each held against the farthest end so far
+static bool items_apart(const az_muon_item* items, i64 n, size_t es) {
+    struct Range { uintptr_t from, to; bool written; };
+    std::vector<Range> all;
+    all.reserve((size_t)n * 3);
+    for (i64 i = 0; i < n; i++) {
+        const size_t count = (size_t)items[i].rows * items[i].cols;
+        const uintptr_t w = (uintptr_t)items[i].w_dev, g = (uintptr_t)items[i].g_dev, m = (uintptr_t)items[i].m_dev;
+        all.push_back({w, w + count * es, true});
+        all.push_back({g, g + count * es, false});
+        all.push_back({m, m + count * 4, true});
+    }
+    std::sort(all.begin(), all.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+    uintptr_t end = 0, written = 0;   // of all, of those written
+    for (const Range& r : all) {
+        if (r.from < (r.written ? end : written)) return false;
+        end = r.to > end ? r.to : end;
+        if (r.written && r.to > written) written = r.to;
+    }
+    return true;
+}
+
 size_t az_muon_step_ws(const az_muon_item* items, int64_t n) {
     size_t most = 0;
     if (!items) return 0;
@@ -937,19 +960,13 @@ int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n
         if (!dims_ok(items[i].rows, items[i].cols)) return refuse("az_muon_step: bad shape (rows and cols are 1..32768)");
         if (!items[i].w_dev || !items[i].g_dev || !items[i].m_dev) return refuse("az_muon_step: null pointer");
     }
-    // what is written (w, m) overlaps nothing else
-    for (int64_t i = 0; i < n; i++) {
-        const size_t ni = (size_t)items[i].rows * items[i].cols, es = dtype_size(dtype);
-        for (int64_t k = 0; k < n; k++) {
-            const size_t nk = (size_t)items[k].rows * items[k].cols;
-            if ((k < i && (overlap(items[i].w_dev, ni * es, items[k].w_dev, nk * es) ||
-                           overlap(items[i].m_dev, ni * 4, items[k].m_dev, nk * 4))) ||
-                overlap(items[i].w_dev, ni * es, items[k].m_dev, nk * 4) ||
-                overlap(items[i].g_dev, ni * es, items[k].w_dev, nk * es) ||
-                overlap(items[i].g_dev, ni * es, items[k].m_dev, nk * 4))
-                return refuse("az_muon_step: weights and momenta must not overlap each other or a gradient");
-        }
+    bool apart = false;
+    try {
+        apart = items_apart(items, n, dtype_size(dtype));
+    } catch (const std::bad_alloc&) {
+        return refuse("az_muon_step: out of host memory");
     }
+    if (!apart) return refuse("az_muon_step: weights and momenta must not overlap each other or a gradient");
     if (!isfinite(lr) || !isfinite(weight_decay) || !(momentum >= 0 && momentum < 1))
         return refuse("az_muon_step: bad lr, weight_decay or momentum (0 <= momentum < 1)");
     int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_muon_step_ws(items, n));

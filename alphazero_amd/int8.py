@@ -73,7 +73,7 @@ def matmul(q, scale, w, w_scale, bias=None, residual=None, act="none", dtype=tor
     """act(scale[m] * w_scale[n] * (q @ w.T)[m, n] + bias[n] + residual[m, n]) of `dtype` [m, n].
 
     q int8 [m, k], w int8 [n, k] with contiguous rows; scale [m], w_scale [n], bias [n] float32; residual [m, n] of `dtype`
-    (may be `out` itself); act: "none", "relu" or "silu".  Integer sums are exact, the rest is float32, rounded once."""
+    (may be `out` itself; `out` overlaps nothing else); act: "none", "relu" or "silu".  Integer sums are exact, the rest is float32, rounded once."""
     if q.dtype is not torch.int8:
         raise AzError("matmul: q must be int8")
     m, k, ld_q = rows_of(q, "matmul", "q")
@@ -97,8 +97,6 @@ def linear(x, w, w_scale, bias=None, residual=None, act="none", out=None):
     dev = same_device("linear", x, w, w_scale, bias, residual, out)
     n, wp, ld_w, out, tail = _layer("linear", m, k, w, w_scale, bias, residual, act, x.dtype, out)
     L, xp = lib(), x.data_ptr()
-    if m * n > 0 and out.data_ptr() == xp:
-        raise AzError("linear: out must not be x")
     nws = L.az_i8_linear_ws(m, n, k, wp, ld_w)
     ws, wsp = workspace(nws, x)
     check(L.az_i8_linear_dev(dev, m, n, k, xp, ld_x, wp, ld_w, *tail, wsp, nws, stream_of(dev)))

@@ -217,6 +217,49 @@ def test_linear_non_finite_rows(I8, m):
         assert torch.equal(y[2], b)
 
 
+def test_columns_of_one_buffer(I8):
+    """output beside input and residual in the rows of one buffer"""
+    from alphazero_amd._abi import AzError
+    buf = torch.randn(50, 200, generator=torch.Generator().manual_seed(3)).cuda()
+    w = torch.randint(-127, 128, (40, 64), dtype=torch.int8, generator=torch.Generator().manual_seed(4)).cuda()
+    s = torch.rand(40, generator=torch.Generator().manual_seed(5)).cuda()
+    x, res, out = buf[:, :64], buf[:, 100:140], buf[:, 64:104 - 4]
+    want = I8.linear(x.clone(), w[:36], s[:36], residual=res[:, :36].clone(), act="relu")
+    kept = buf.clone()
+    y = I8.linear(x, w[:36], s[:36], residual=res[:, :36], act="relu", out=out)
+    assert torch.equal(y, want) and y.data_ptr() == out.data_ptr()
+    kept[:, 64:100] = want
+    assert torch.equal(buf, kept)
+    with pytest.raises(AzError, match="overlap"):
+        I8.linear(x, w[:36], s[:36], out=buf[:, 40:76])
+    with pytest.raises(AzError, match="residual"):
+        I8.linear(x, w[:36], s[:36], residual=buf[:, 80:116], out=out)
+
+
+def test_offsets_past_32_bits(I8):
+    """3 GB of 8-bit rows on either side, 5.6 GB of output"""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randint(-127, 128, (50000, 60000), dtype=torch.int8, device="cuda", generator=gen)
+    w = torch.randint(-127, 128, (70, 60000), dtype=torch.int8, device="cuda", generator=gen)
+    one = torch.ones(70000, device="cuda")
+    at = [0, 17000, 35791, 35792, 49999]
+    want = (q[at].double().unsqueeze(1) * w.double()).sum(2)          # exact; a float32 result is its rounding
+    assert torch.equal(I8.matmul(q, one[:50000], w, one[:70])[at], want.float())
+    assert torch.equal(I8.matmul(w, one[:70], q, one[:50000])[:, at], want.float().t())
+    del q, w
+    x = torch.empty(40000, 60000, dtype=torch.float16, device="cuda").normal_(generator=gen)
+    r, s = I8.quantize_rows(x, torch.tensor([[39999], [35792], [0], [40000]], dtype=torch.int32, device="cuda"))
+    assert torch.equal(r[:3].double(), torch.round(x[[39999, 35792, 0]].double() / s[:3].double().unsqueeze(1)))
+    assert (r[3] == 0).all() and s[3] == 0
+    r, s = I8.quantize_rows(x)
+    assert torch.equal(r[at[:4]].double(), torch.round(x[at[:4]].double() / s[at[:4]].double().unsqueeze(1)))
+    del x, r
+    a = torch.randint(-127, 128, (70000, 48), dtype=torch.int8, device="cuda", generator=gen)
+    y = I8.matmul(a, one, a[:40000], one[:40000], dtype=torch.bfloat16)
+    for i in (0, 53687, 69999):
+        assert torch.equal(y[i], (a[i].double() * a[:40000].double()).sum(1).to(torch.bfloat16))
+
+
 def test_empty_calls(I8):
     w, ws = torch.zeros(5, 8, dtype=torch.int8).cuda(), torch.ones(5).cuda()
     assert I8.matmul(w[:0], ws[:0], w, ws).shape == (0, 5)

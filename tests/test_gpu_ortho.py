@@ -84,6 +84,15 @@ def test_wide_matrices_of_low_rank(O, steps, noise):
         assert float((y.cpu().double() - want).norm()) <= tol
 
 
+@pytest.mark.parametrize("coeffs", [(2.0, -1.5, 0.5), (1.875, -1.25, 0.375), (3.0, -3.2, 1.2), (4.1, -6.9, 2.95), (-1.5, 0.5, 0.0)])
+@pytest.mark.parametrize("steps", [3, 5, 9])
+def test_wide_matrices_with_other_coefficients(O, coeffs, steps):
+    g = gradient(140, 1200, steps)
+    y = O.orthogonalize(g.cuda(), steps=steps, coeffs=coeffs)
+    want, tol = allowed(g, torch.float32, steps=steps, coeffs=coeffs)
+    assert float((y.cpu().double() - want).norm()) <= tol
+
+
 def test_cubic_iteration_converges_to_the_polar_factor(O):
     g = torch.linalg.qr(torch.randn(90, 60, dtype=torch.float64, generator=torch.Generator().manual_seed(1)))[0]
     g = g @ torch.diag(torch.linspace(0.5, 1.0, 60, dtype=torch.float64)) @ torch.linalg.qr(torch.randn(60, 60, dtype=torch.float64))[0]
@@ -106,7 +115,7 @@ def test_batches_of_all_lengths_and_dimensions(O):
 
 
 def test_zero_nan_tiny_and_huge_matrices(O):
-    for rows, cols in ((30, 50), (150, 140)):
+    for rows, cols in ((30, 50), (150, 140), (700, 140)):
         g = torch.stack([gradient(rows, cols, i) for i in range(7)])
         g[0] = 0
         g[1, 3, 4] = float("nan")
@@ -122,6 +131,24 @@ def test_zero_nan_tiny_and_huge_matrices(O):
             want = plain(g[i].double(), eps=1e-30)
             _, tol = allowed(scaled, torch.float32, eps=1e-30)
             assert float((y[i].double() - want).norm()) <= tol
+
+
+@pytest.mark.parametrize("rows,cols", [(17000, 32768), (32768, 17000)])
+def test_offsets_past_32_bits(O, rows, cols):
+    """one value in each row and column: the iteration of numbers, in 2.2 GB"""
+    s, gen = min(rows, cols), torch.Generator().manual_seed(rows)
+    i, j = torch.randperm(rows, generator=gen)[:s].cuda(), torch.randperm(cols, generator=gen)[:s].cuda()
+    v = torch.randn(s, generator=gen).cuda()
+    g = torch.zeros(rows, cols, device="cuda")
+    g[i, j] = v
+    y = O.orthogonalize(g, out=g)
+    x = v.double() / (v.double().norm() + 1e-7)
+    for _ in range(5):
+        x = x * (3.4445 - 4.7750 * x ** 2 + 2.0315 * x ** 4)
+    got = y[i, j].double()
+    assert float((got - x).norm()) <= 8 * 64 * U * float(x.norm())
+    y[i, j] = 0
+    assert not y.any()
 
 
 def test_in_place_strided_input_streams_and_graphs(O):

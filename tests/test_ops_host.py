@@ -70,6 +70,39 @@ def test_matmul_refuses():
     assert L.az_i8_linear_ws(4, 6, 0, P, 8) == 0 and L.az_i8_matmul_ws(4, 6, 8, P, 8, P, 8) == 0
 
 
+def test_int8_outputs_overlap_nothing():
+    L = _abi.lib()
+    at = {"x": 0x100000, "xs": 0x200000, "w": 0x300000, "ws": 0x400000, "bias": 0x500000, "res": 0x600000, "y": 0x700000}
+
+    def call(fn, m=4, n=6, k=8, ld_x=8, ld_w=8, ld_res=6, ld_y=6, **over):
+        a = {name: C.c_void_p(p) for name, p in {**at, **over}.items()}
+        if fn == "matmul":
+            return L.az_i8_matmul_dev(0, m, n, k, a["x"], ld_x, a["xs"], a["w"], ld_w, a["ws"], a["bias"], a["res"], ld_res, 0, 0,
+                                      a["y"], ld_y, P, 1 << 20, None)
+        return L.az_i8_linear_dev(0, m, n, k, a["x"], ld_x, a["w"], ld_w, a["ws"], a["bias"], a["res"], ld_res, 0, 0, a["y"], ld_y,
+                                  P, 1 << 20, None)
+
+    for fn in ("matmul", "linear"):
+        for name in ("x", "w", "ws", "bias") + (("xs",) if fn == "matmul" else ()):
+            _refused(call(fn, y=at[name]), "overlap")
+            _refused(call(fn, y=at[name] - 92), "overlap")              # y is 96 bytes
+        _refused(call(fn, res=at["y"] + 4), "residual")
+        _refused(call(fn, res=at["y"], ld_res=12), "residual")
+        _refused(call(fn, res=at["y"] + 20, ld_y=12, ld_res=12), "residual")     # columns 5..10 beside 0..5
+        _refused(call(fn, res=at["y"] + 28, ld_y=12, ld_res=12), "residual")     # columns 7..12: into the next row
+        if _abi.device_count() == 0:
+            for kw in (dict(), dict(res=at["y"]), dict(y=at["x"] - 96), dict(res=at["y"] + 24, ld_y=12, ld_res=12),
+                       dict(res=at["y"] - 24, ld_y=12, ld_res=12), dict(m=1, res=at["y"], ld_res=99)):
+                assert call(fn, **kw) == NO_DEVICE
+    def quantize(x=0x1000, q=0x8000, s=0x9000, index=0xa000):
+        return L.az_i8_quantize_dev(0, 0, 4, 8, C.c_void_p(x), 8, 5, C.c_void_p(index), 2, C.c_void_p(q), 16, C.c_void_p(s), None)
+
+    for kw in (dict(q=0x1000), dict(q=0x1000 + 156), dict(s=0x1000), dict(s=0x8004), dict(index=0x8000), dict(index=0x9008)):
+        _refused(quantize(**kw), "overlap")
+    if _abi.device_count() == 0:
+        assert quantize() == NO_DEVICE and quantize(q=0x1000 + 160) == NO_DEVICE
+
+
 def test_ortho_refuses():
     L = _abi.lib()
     good = (3.4445, -4.7750, 2.0315)
@@ -116,6 +149,11 @@ def test_muon_refuses():
     _refused(call([(0x1000, 0x1000, 0x3000, 4, 4)]), "overlap")            # the gradient is the weight
     _refused(call([(0x1000, 0x2000, 0x1000, 4, 4)]), "overlap")            # so is the momentum
     _refused(call([one, (0x4000, 0x5000, 0x2000, 4, 4)]), "overlap")       # another item's gradient is the momentum
+    many = [(0x10000 + 0x300 * i, 0x10100 + 0x300 * i, 0x10200 + 0x300 * i, 4, 4) for i in range(3000)]
+    _refused(call(many + [(0x10000 + 0x300 * 1234 + 0x20, 0x900000, 0xa00000, 4, 4)]), "overlap")
+    _refused(call([(0x10000, 0x20000, 0x30000, 64, 64), (0x100000, 0x10100, 0x200000, 4, 4)]), "overlap")   # inside a long one
+    if _abi.device_count() == 0:
+        assert call(many) == NO_DEVICE
     _refused(call([(0, 0x2000, 0x3000, 4, 4)]), "null")
     _refused(call([(0x1000, 0x2000, 0x3000, 0, 4)]), "shape")
     _refused(call([one], lr=float("nan")), "lr")
