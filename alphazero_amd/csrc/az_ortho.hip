@@ -808,21 +808,27 @@ static int run_jobs(Jobs& all, const Hyper& h, int steps, int dtype, hipStream_t
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
-    // steps on the s x s side where that is less work in all
-    int len[16], n = 0, left = steps;
-    double one_by_one = 0, several = 0;
+    // Steps on the s x s side where that should take less time.  A launch costs 5 us and its work at 0.9 PFLOP/s, or 0.1 us for
+    // every 16 values of the sums of its longest tile (both as measured, a symmetric product as 0.8 of a whole one).  2 + 3 | one by one,
+    // us: 2 x 333 x 1027 155 | 151, 2 x 400 x 800 158 | 147, 1024 x 1536 251 | 247, 1024 x 2048 264 | 273, 300 x 2000 151 | 167,
+    // 512 x 4096 211 | 272, 1024 x 4096 309 | 377
+    int len[16], n = 0, left = steps, squares = 0;
     while (left > 0) {
         len[n] = n == 0 ? (left < 2 ? left : 2) : (left < 3 ? left : 3);
+        squares += len[n] == 1 ? 0 : len[n] == 2 ? 3 : 6;
         left -= len[n++];
     }
+    double s2l = 0, s3 = 0, longest_l = 0, longest_s = 0;
     for (int i = 0; i < js.n; i++) {
         const double s = js.j[i].sp, l = js.j[i].lp;
-        one_by_one += steps * (1.8 * s * s * l + 0.8 * s * s * s);
-        for (int k = 0; k < n; k++) several += 1.8 * s * s * l + 0.8 * s * s * s * (len[k] == 1 ? 1 : len[k] == 2 ? 5 : 9);
+        s2l += s * s * l;
+        s3 += s * s * s;
+        longest_l = fmax(longest_l, l);
+        longest_s = fmax(longest_s, s);
     }
-    // 2 + 3 is 18 launches against 15.  Measured, 2 + 3 | one by one: 1024 x 1536 251 | 247 us (0.95 of the work), 2 x 400 x 800
-    // 158 | 147 and 1024 x 2048 264 | 273 (0.84), 300 x 2000 151 | 167 (0.57), 1024 x 4096 309 | 377 (0.64)
-    if (several > 0.8 * one_by_one || steepest(h, steps) > 16.0)
+    auto launch = [](double products, double k) { return 5.0 + fmax(6 * products / 0.9e9, 0.1 * k / 16); };
+    const double on_x = launch(0.8 * s2l, longest_l) + launch(s2l, longest_s), on_a = launch(0.8 * s3, longest_s);
+    if (n * on_x + (steps + squares) * on_a > steps * (on_x + on_a) || steepest(h, steps) > 16.0)
         for (n = 0; n < steps; n++) len[n] = 1;
     const Op gram = {0, 0, 0, 0x1p-16f};                                  // 2^14 2^14 -> 2^12
     auto poly = [](int out) { return Op{0, 0, out, 0x1p-24f}; };           // 2^12 2^12 -> 1, then 2^11
