@@ -328,12 +328,13 @@ using OTile64 = TileShape<64, 64, 2, 2, 3, 4>;   // few tiles: what counts is th
 // launch adds up the panels' parts of A = X X^T (in order, so the sum is the same every time); in the second every workgroup owns
 // some panels and
 //   1. takes A into LDS,
-//   2. makes B = a I + b A + c A A^T for itself,
+//   2. makes B = a I + b A + c A A^T for itself, and as a rule the next step's as well, of B A B (two steps a launch),
 //   3. multiplies its panels by it, keeping T for the next launch, and adds up their part of the next Gram matrix.
 // What bounds it is latency: 5 steps of a 128 x 1152 matrix are 0.4 GFLOP, but 15 products one after the other; between launches,
-// each product would start on cold operands.  Seven matrices up to 128 x 1152 in one call: norm 6 us, init 13, sums 4 a step, steps
-// 15 (the last 12.6), 104 us in all (us, this form | the wide matrices': 104 | 136; alone, 128 x 1152 93 | 104, 128 x 32768 231 | 483,
-// 4 x 100 x 5000 136 | 181, 16 x 64 x 64 65 | 77, 128 x 128 91 | 76).
+// each product would start on cold operands.  Seven matrices up to 128 x 1152 in one call: norm 6 us, init 12, sums 4.5 a launch, two
+// steps 24 (2.5 for each of the four products more, which read 512 KB of LDS; one step is 14.8), the last alone 12: 89 us in all, 104 with
+// one step a launch (us, this form | the wide matrices': 89 | 136; alone, 128 x 1152 81 | 104, 128 x 32768 173 | 483, 4 x 100 x 5000
+// 108 | 181, 16 x 64 x 64 50 | 77, 128 x 128 80 | 76).
 //
 // T goes through memory in the order in which the MFMA of 3. takes it and the one before leaves it.  D = B T^T leaves lane
 // (h = lane / 32, j = lane % 32) rows i = 8 (r / 4) + 4 h + r % 4 of column j: eight registers are eight values of k for lane (h, j) of the
@@ -500,8 +501,12 @@ __global__ __launch_bounds__(256) void k_narrow_sum(Jobs js) {
         for (int e = 0; e < 4; e++) nar_put(J.image, m + e, swap23(n), v[e]);
 }
 
-template <class T, bool LASTSTEP>
-__global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int cur) {
+// TWO: two steps.  The powers of two from the sums to P, and from P X to X (to the output in the last launch)
+struct Narrow {
+    float p_unit, x_unit;
+};
+template <class T, bool LASTSTEP, bool TWO>
+__global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int cur, Narrow pass) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     u8 *const bufA = lds, *const bufB = lds + NBUF;   // A, then the new panel; B
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -539,7 +544,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(bufT + ((jb * 4 + ib) * 2 + low) * 1024), 16, lane * 16, low * 1024, 0, 0);
     };
     fetch_high(first);
-    fetch(first);
+    if (!TWO) fetch(first);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     // 2. B, every block of it
@@ -559,6 +564,41 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
         }
     }
     __syncthreads();
+    if constexpr (TWO) {   // P = B2 B instead of B, with B2 = f(B A B)
+        const bool on = wave < J.nb * J.nb;
+        const int bi = wave / J.nb * 32, bj = (wave - wave / J.nb * J.nb) * 32, n = bj + (lane & 31);
+        // a product of two of these symmetric, commuting matrices, into a buffer that it reads itself
+        auto times = [&](const u8* P, const u8* Q, u8* out, float unit, bool poly) {
+            f32x16 acc = {};
+            if (on) {
+                nar_block(P, bi, Q, bj, steps, lane, acc);
+                acc *= unit;
+                if (poly)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        const int m = bi + acc_row(4 * g, lane);
+                        float v[4];
+                        nar_get4(P, m, n, v);
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            acc[4 * g + e] = (h.c * acc[4 * g + e] + h.b * (v[e] * 0x1p-12f) + (m + e == n ? h.a : 0.0f)) * 0x1p11f;
+                    }
+            }
+            __syncthreads();
+            if (on)
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const float v[4] = {acc[4 * g], acc[4 * g + 1], acc[4 * g + 2], acc[4 * g + 3]};
+                    nar_put4(out, bi + acc_row(4 * g, lane), n, v);
+                }
+            __syncthreads();
+        };
+        times(bufA, bufB, bufA, 0x1p-11f, false);
+        times(bufA, bufB, bufA, 0x1p-11f, false);
+        times(bufA, bufA, bufA, 0x1p-24f, true);
+        fetch(first);   // not earlier: its 32 registers spill others
+        times(bufA, bufB, bufB, pass.p_unit, false);
+    }
     // 3. the panels
     f32x16 gram = {};
     for (int p = first; p < end; p++) {
@@ -584,7 +624,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
             }
             acc += cross;
             if (!LASTSTEP) {
-                acc *= 0x1p-11f;
+                acc *= pass.x_unit;
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     f16x8 hi, lo;
@@ -615,7 +655,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
                 for (int r = 0; r < 16; r++) {
                     const int row = row0 + acc_row(r, lane);
                     if (row >= J.rows || col >= J.cols) continue;
-                    float o = acc[r] * 0x1p-25f;
+                    float o = acc[r] * pass.x_unit;
                     if (h.update) o = old[r] * h.decay - o * (h.lr * J.kappa);
                     ((T*)J.w)[(i64)row * J.cols + col] = from_f32<T>(o);
                 }
@@ -784,11 +824,25 @@ static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_
     const dim3 grid(most, js.n), block(NTHREADS);
     AZ_DISPATCH_DTYPE(dtype, k_narrow_init<T><<<grid, block, NBUF, st>>>(js, h));
     const dim3 grid_sum(10, js.n);   // blocks of a 128 x 128 matrix's lower triangle
-    for (int it = 0; it < steps; it++) {
+    const bool pairs = steepest(h, steps) <= 16.0;
+    int cur = 0;
+    for (int done = 0; done < steps; cur ^= 1) {
+        const bool two = pairs && done + 2 <= steps;
+        const int e = two ? product_exponent(h, done, 2) : 11;
+        done += two ? 2 : 1;
+        const bool last = done == steps;
+        const Narrow pass = {ldexpf(1.0f, e - 22), ldexpf(1.0f, last ? -14 - e : -e)};
         k_narrow_sum<<<grid_sum, dim3(256), 0, st>>>(js);
-        if (it + 1 < steps) k_narrow_step<float, false><<<grid, block, NSTEP_LDS, st>>>(js, h, it & 1);
+        if (last && two) {
+            AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true, true><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass));
+        } else if (last) {
+            AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true, false><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass));
+        } else if (two) {
+            k_narrow_step<float, false, true><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass);
+        } else {
+            k_narrow_step<float, false, false><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass);
+        }
     }
-    AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true><<<grid, block, NSTEP_LDS, st>>>(js, h, (steps - 1) & 1));
     return launch_status("az_orthogonalize");
 }
 
