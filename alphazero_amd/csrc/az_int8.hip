@@ -164,8 +164,8 @@ __device__ inline u32 lanes_max(u32 v) {
 // LANES lanes to a row, NP pieces of 16 bytes to a lane: the row is read once and stays in registers between its largest
 // magnitude and its integers.  FAST: the columns are whole pieces, rows are 16-byte aligned, offsets fit 31 bits and the factors
 // of a row's offset 24 (full-rate multiplications); rows that are not there are read behind the end of the buffer, as zeros.
-// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 43 us, 2.8 TB/s of the 5.1 that a copy reaches; the VALU is busy for two
-// thirds of it (the exact quotient, its tie, the packing).  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
+// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 40 us, 3.0 TB/s of the 5.1 that a copy reaches; what bounds it is the VALU
+// (40 instructions for 8 values: the quotient, how near a half it is, the packing) beside two trips to memory, index and rows.  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
 // One row of 4096 bf16: 3.6 us, all of it latency: the load, the reduction over 4 waves, the launch.
 template <class T, int LANES, int NP, bool FAST>
 __global__ __launch_bounds__(256) void k_i8_quantize(Rows R) {
@@ -228,19 +228,19 @@ __global__ __launch_bounds__(256) void k_i8_quantize(Rows R) {
         if (R.fill)
             for (i64 c = R.taps * R.cols + l; c < R.ld_q; c += LANES) q[c] = 0;
         u32 again = 0;   // pieces to do over the exact way
+        const u32 keep = s >= QUANT_TINY ? ~0u : 0u;   // else s is 0, NaN or tiny
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             if (l + i * LANES >= R.pieces) continue;
             u32 out[EPP / 4];
-            const bool fine = v[i].quantize(rs, out);
-            if (!(s >= QUANT_TINY)) {   // s is 0, NaN or tiny
+            again |= v[i].quantize(rs, out) ? 0u : 1u << i;
 #pragma unroll
-                for (int e = 0; e < EPP / 4; e++) out[e] = 0;
-                again |= s > 0 ? 1u << i : 0;
-            } else if (!fine) {
-                again |= 1u << i;
-            }
+            for (int e = 0; e < EPP / 4; e++) out[e] &= keep;
             piece_store<T>(q + (FAST ? (l + i * LANES) * EPP : to[i]), out, FAST ? EPP : n[i]);
+        }
+        if (!keep) {
+            again = 0;
+            for (int i = 0; i < NP && s > 0; i++) again |= l + i * LANES < R.pieces ? 1u << i : 0u;
         }
         while (again) {   // one copy of the code: about one piece in 2000 comes here
             const int i = __builtin_ctz(again);
