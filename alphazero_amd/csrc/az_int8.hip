@@ -6,6 +6,8 @@
 // The sums are int32 and exact (|q w| <= 2^14, k <= 131071), so no order of summation changes a result.
 #include <math.h>
 
+#include <type_traits>
+
 #include "az_tile.hpp"
 
 namespace az {
@@ -385,78 +387,99 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
     const u32 first = blockIdx.y * steps_per_split;
     u32 kend = (first + steps_per_split) * TILE_KB;
     kend = kend < (u32)p.k ? kend : (u32)p.k;
+    // scales of the tile's rows and columns: asked for before the product, which they arrive under, and handed out through LDS
+    static_assert(S::THREADS >= S::BM && S::THREADS >= S::BN, "a value a thread");
+    const int t = threadIdx.x;
+    const float scale_m = p.qs[m0 + t < p.m ? m0 + t : p.m - 1];
+    const i64 nt = n0 + t < p.n ? n0 + t : p.n - 1;
+    const float scale_n = p.ws[nt], bias_n = p.bias ? p.bias[nt] : 0.0f;
     i32x16 acc[S::FM][S::FN] = {};
     tile_product<KindI8, S>(KindI8(), a, b, first, kend, lds, wave, lane, acc);
-    // scales of the tile's rows and columns through LDS (its tiles have been read)
-    float *sm = (float*)lds, *sn = sm + S::BM, *bn = sn + S::BN;
-    for (int t = threadIdx.x; t < S::BM; t += S::THREADS) sm[t] = p.qs[m0 + t < p.m ? m0 + t : p.m - 1];
-    for (int t = threadIdx.x; t < S::BN; t += S::THREADS) {
-        const i64 n = n0 + t < p.n ? n0 + t : p.n - 1;
-        sn[t] = p.ws[n];
-        bn[t] = p.bias ? p.bias[n] : 0.0f;
-    }
-    __syncthreads();
     const int wm = wave / S::WN * (S::FM * 32), wn = wave % S::WN * (S::FN * 32);
+    const int rows = (int)(p.m - m0 < S::BM ? p.m - m0 : S::BM);
     constexpr int W = S::PAIRS ? 2 : 1;   // neighbouring columns a lane holds
-    if (part) part += (i64)blockIdx.y * p.m * p.n;
+    if (part) {
+        part += (i64)blockIdx.y * p.m * p.n;
 #pragma unroll
-    for (int j = 0; j < S::FN; j += W) {
-        const int c = wn + 32 * j + W * (lane & 31);
-        const i64 n = n0 + c;
-        const float s0 = sn[c], b0 = bn[c], s1 = sn[c + W - 1], b1 = bn[c + W - 1];
-        const bool two = W == 2 && n + 1 < p.n;
-        if (n >= p.n) continue;
+        for (int j = 0; j < S::FN; j += W) {
+            const i64 n = n0 + wn + 32 * j + W * (lane & 31);
+            if (n >= p.n) continue;
 #pragma unroll
-        for (int i = 0; i < S::FM; i++) {
-            float res[16][W];
-            if (p.res && !part) {   // a block's residuals on their way at once
-                T raw[16][W];
+            for (int i = 0; i < S::FM; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
-                    const i64 m = m0 + wm + 32 * i + acc_row(r, lane);
-                    const T* s = (const T*)p.res + (m < p.m ? m : p.m - 1) * p.ld_res + n;
-                    raw[r][0] = s[0];
-                    if (W == 2) raw[r][W - 1] = s[two ? 1 : 0];
+                    const int row = wm + 32 * i + acc_row(r, lane);
+                    if (row >= rows) continue;
+                    part[(m0 + row) * p.n + n] = acc[i][j][r];
+                    if (W == 2 && n + 1 < p.n) part[(m0 + row) * p.n + n + 1] = acc[i][j + W - 1][r];
                 }
-                loads_first();
+        }
+        return;
+    }
+    float *sm = (float*)lds, *sn = sm + S::BM, *bn = sn + S::BN;   // its tiles have been read
+    if (t < S::BM) sm[t] = scale_m;
+    if (t < S::BN) {
+        sn[t] = scale_n;
+        bn[t] = bias_n;
+    }
+    __syncthreads();
+    auto finish = [&](auto act) {   // a copy for each activation: no branch between the values
 #pragma unroll
-                for (int r = 0; r < 16; r++)
+        for (int j = 0; j < S::FN; j += W) {
+            const int c = wn + 32 * j + W * (lane & 31);
+            const i64 n = n0 + c;
+            const float s0 = sn[c], b0 = bn[c], s1 = sn[c + W - 1], b1 = bn[c + W - 1];
+            const bool two = W == 2 && n + 1 < p.n;
+            if (n >= p.n) continue;
 #pragma unroll
-                    for (int k = 0; k < W; k++) res[r][k] = to_f32(raw[r][k]);
-            } else {
+            for (int i = 0; i < S::FM; i++) {
+                float res[16][W];
+                if (p.res) {   // a block's residuals on their way at once
+                    T raw[16][W];
 #pragma unroll
-                for (int r = 0; r < 16; r++)
-#pragma unroll
-                    for (int k = 0; k < W; k++) res[r][k] = -0.0f;   // adds nothing, not even a sign
-            }
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-                const int row = wm + 32 * i + acc_row(4 * g, lane);
-                const f32x4 s4 = *(const f32x4*)(sm + row);
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const i64 m = m0 + row + e;
-                    if (m >= p.m) break;
-                    const int q0 = acc[i][j][4 * g + e], q1 = acc[i][j + W - 1][4 * g + e];
-                    if (part) {
-                        part[m * p.n + n] = q0;
-                        if (two) part[m * p.n + n + 1] = q1;
-                        continue;
+                    for (int r = 0; r < 16; r++) {
+                        const i64 m = m0 + wm + 32 * i + acc_row(r, lane);
+                        const T* s = (const T*)p.res + (m < p.m ? m : p.m - 1) * p.ld_res + n;
+                        raw[r][0] = s[0];
+                        if (W == 2) raw[r][W - 1] = s[two ? 1 : 0];
                     }
-                    float v0 = (float)q0 * s4[e] * s0 + b0 + res[4 * g + e][0], v1 = (float)q1 * s4[e] * s1 + b1 + res[4 * g + e][W - 1];
-                    T* y = (T*)p.y + m * p.ld_y + n;
-                    v0 = activate<T>(v0, p.act);
-                    if (two && p.pair_store) {
-                        struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
-                        *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate<T>(v1, p.act))};
-                    } else {
-                        y[0] = from_f32<T>(v0);
-                        if (two) y[1] = from_f32<T>(activate<T>(v1, p.act));
+                    loads_first();
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+#pragma unroll
+                        for (int k = 0; k < W; k++) res[r][k] = to_f32(raw[r][k]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+#pragma unroll
+                        for (int k = 0; k < W; k++) res[r][k] = -0.0f;   // adds nothing, not even a sign
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    const int row = wm + 32 * i + acc_row(4 * g, lane);
+                    const f32x4 s4 = *(const f32x4*)(sm + row);
+                    T* y = (T*)p.y + (m0 + row) * p.ld_y + n;
+#pragma unroll
+                    for (int e = 0; e < 4; e++, y += p.ld_y) {
+                        if (row + e >= rows) break;
+                        const int q0 = acc[i][j][4 * g + e], q1 = acc[i][j + W - 1][4 * g + e];
+                        float v0 = (float)q0 * s4[e] * s0 + b0 + res[4 * g + e][0], v1 = (float)q1 * s4[e] * s1 + b1 + res[4 * g + e][W - 1];
+                        v0 = activate<T>(v0, act);
+                        if (two && p.pair_store) {
+                            struct __attribute__((aligned(2 * sizeof(T)))) Two { T a, b; };
+                            *(Two*)y = Two{from_f32<T>(v0), from_f32<T>(activate<T>(v1, act))};
+                        } else {
+                            y[0] = from_f32<T>(v0);
+                            if (two) y[1] = from_f32<T>(activate<T>(v1, act));
+                        }
                     }
                 }
             }
         }
-    }
+    };
+    if (p.act == AZ_ACT_SILU) finish(std::integral_constant<int, AZ_ACT_SILU>());
+    else if (p.act == AZ_ACT_RELU) finish(std::integral_constant<int, AZ_ACT_RELU>());
+    else finish(std::integral_constant<int, AZ_ACT_NONE>());
 }
 // the parts' sums, and the product's epilogue: 128 x 128 x 4096 in 8 parts, with the tiles, 9.3 us
 template <class T>
