@@ -166,7 +166,7 @@ __device__ inline u32 lanes_max(u32 v) {
 // LANES lanes to a row, NP pieces of 16 bytes to a lane: the row is read once and stays in registers between its largest
 // magnitude and its integers.  FAST: the columns are whole pieces, rows are 16-byte aligned, offsets fit 31 bits and the factors
 // of a row's offset 24 (full-rate multiplications); rows that are not there are read behind the end of the buffer, as zeros.
-// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 40 us, 3.0 TB/s of the 5.1 that a copy reaches; what bounds it is the VALU
+// 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 37 us, 3.3 TB/s of the 5.1 that a copy reaches; what bounds it is the VALU
 // (40 instructions for 8 values: the quotient, how near a half it is, the packing) beside two trips to memory, index and rows.  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
 // One row of 4096 bf16: 3.6 us, all of it latency: the load, the reduction over 4 waves, the launch.
 template <class T, int LANES, int NP, bool FAST>
@@ -367,10 +367,10 @@ __device__ inline void put(const Mm& p, i64 m, i64 n, int sum, float scale) {
 
 // Rows of both operands at multiples of 16 bytes, k a multiple of 16.  blockIdx.y: which of the `splits` parts of k (whole
 // steps each); with more than one the int32 sums go to part[split][m][n] and k_i8_join adds them.
-// 8192^3, 256 x 256 tiles: 532-576 us, 1.9-2.1 POP/s of the 2.5 that the library's product reaches; the matrix pipe is busy for 59 % at
-// 1.66 GHz (power): a k slice costs as many LDS cycles as MFMA cycles.  86016 x 128 x 1152, 128 x 128 tiles: 33 us, 3.7 TB/s of the
-// rows it has to read, with SiLU and fp16 stores.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 9.2 us, one after the other:
-// launch, first tiles, 17 steps, scales and residual, stores.
+// 8192^3, 256 x 256 tiles: 545 us, 2.0 POP/s of the 2.5 that the library's product reaches; the matrix pipe is busy for 59 % at
+// 1.66 GHz (power): a k slice costs as many LDS cycles as MFMA cycles.  86016 x 128 x 1152, 128 x 128 tiles: 29 us, 4.2 TB/s of rows
+// read and results written, SiLU on the way.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 7.8 us, one after the other:
+// launch, first tiles, 17 steps, residual, stores.
 template <class T, class S>
 __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u32 tiles_n, u32 steps_per_split, int* part) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
     else if (p.act == AZ_ACT_RELU) finish(std::integral_constant<int, AZ_ACT_RELU>());
     else finish(std::integral_constant<int, AZ_ACT_NONE>());
 }
-// the parts' sums, and the product's epilogue: 128 x 128 x 4096 in 8 parts, with the tiles, 9.3 us
+// the parts' sums, and the product's epilogue: 128 x 128 x 4096 in 4 parts, with the tiles, 7.9 us
 template <class T>
 __global__ __launch_bounds__(256) void k_i8_join(Mm p, u32 splits, const int* __restrict__ part) {
     const i64 total = p.m * p.n;
@@ -651,13 +651,15 @@ static i64 up(i64 n, i64 to) { return (n + to - 1) / to * to; }
 
 // When k_i8_mm_few takes a product of up to 64 rows.  It reads q from L2 once for every 16 channels, the tiles once for every 64, and
 // splits k over 8 waves only, the tiles over 16 workgroups; but it is one launch and takes rows at any address, which the tiles
-// need copied first (us, few | tiles: 1 x 4096 x 4096 5.0 | 8.4, 16 x 4096 x 4096 6.4 | 9.4, 16 x 8192 x 8192 17.5 | 16.2,
-// 16 x 128 x 16384 16.1 | 10.9, 32 x 4096 x 4096 8.3 | 10.3, 32 x 8192 x 8192 24.8 | 17.4, 42 x 128 x 1152 4.5 | 7.2,
-// 64 x 1024 x 1024 5.0 | 7.2, 64 x 4096 x 4096 12.1 | 11.2, 64 x 8192 x 8192 38.7 | 18.7).
+// need copied first (us, few | tiles: 1 x 4096 x 4096 5.3 | 7.7, 1 x 8192 x 8192 12.4 | 14.7, 8 x 8192 x 8192 14.4 | 15.3, 16 x 4096 x 4096
+// 6.3 | 8.5, 16 x 4096 x 8192 9.8 | 11.0, 16 x 8192 x 8192 17.2 | 15.5, 16 x 128 x 16384 15.9 | 10.2, 32 x 4096 x 4096 8.3 | 9.1,
+// 32 x 1024 x 4096 7.7 | 8.1, 24 x 512 x 8192 11.4 | 9.0, 32 x 8192 x 8192 24.9 | 16.2, 42 x 128 x 1152 4.5 | 5.2, 48 x 4096 x 1024 4.7 | 5.1,
+// 48 x 1024 x 4096 9.6 | 8.3, 64 x 2048 x 2048 7.2 | 7.1, 64 x 4096 x 4096 12.3 | 10.2).
 static bool few_rows(i64 m, i64 n, i64 k, bool aligned) {
     if (m > 64) return false;
     if (!aligned) return true;
-    return k <= 8192 && (m <= 16 || n * k <= (m <= 32 ? 16 << 20 : 8 << 20));
+    if (m <= 16) return k <= 8192 && (m <= 8 || n * k <= 32 << 20);
+    return m <= 32 ? k <= 4096 && n * k <= 16 << 20 : k <= 2048 && n * k <= 4 << 20;
 }
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
@@ -688,14 +690,14 @@ static MmPlan mm_plan(i64 m, i64 n, i64 k, const void* q, i64 ld_q, bool q_padde
     P.w_bytes = P.align_w ? up256((size_t)n * P.kp) : 0;
     auto tiles = [&](i64 e) { return ((m + e - 1) / e) * ((n + e - 1) / e); };
     // A larger tile reads less per product, but must not be mostly padding and must fill the chip: at least 200 of them (us; with
-    // 400 or 100 instead: 2048^3 17.2 | 22.8 with 400, 3000 x 3000 x 512 16.7 | 26.8 with 100).
+    // 400 or 100 instead: 2048^3 15.3 | 19.3 with 400, 3000 x 3000 x 512 15.8 | 20.9 with 100).
     auto pays = [&](i64 e) { return tiles(e) >= 200 && tiles(e) * e * e <= tiles(e / 2) * (e / 2) * (e / 2) * 9 / 8; };
     P.tile = pays(256) ? 256 : pays(128) ? 128 : 64;
-    // k split over workgroups where the tiles are too few for the CUs, in parts of at least 16 steps (us, split | not:
-    // 65 x 64 x 8192 10.2 | 19.6, 128 x 128 x 4096 9.3 | 12.6, 256 x 256 x 2048 8.8 | 9.1)
+    // k split over workgroups where the tiles are too few for the CUs, from 64 steps on, in parts of at least 16 (us, split | not:
+    // 65 x 64 x 8192 8.9 | 15.6, 128 x 128 x 4096 7.9 | 9.6, 70 x 1000 x 4096 8.4 | 9.7, 65 x 64 x 3200 8.1 | 8.0, 256 x 256 x 2048 7.6 | 6.6)
     const u32 steps = (u32)((k + TILE_KB - 1) / TILE_KB);
     u32 splits = 1;
-    if (P.tile == 64)
+    if (P.tile == 64 && steps >= 64)
         while (splits < 16 && tiles(64) * splits * 2 <= 256 && steps / (splits * 2) >= 16) splits *= 2;
     P.steps_per_split = (steps + splits - 1) / splits;
     P.splits = (steps + P.steps_per_split - 1) / P.steps_per_split;

@@ -131,7 +131,8 @@ def operands(m, n, k, seed, dt, bias=True, res=False, full=False):
 SHAPES = [(1, 1, 1), (1, 1, 129), (1, 7, 126), (2, 3, 42), (1, 128, 1152), (1, 1003, 4096), (3, 129, 27), (5, 64, 4097), (16, 256, 512),
           (17, 31, 64), (31, 33, 128), (42, 128, 1152), (63, 65, 127), (64, 64, 16), (65, 1, 1000), (84, 128, 252),
           (127, 129, 144), (128, 128, 128), (129, 257, 272), (300, 500, 1031), (256, 256, 2048), (257, 511, 384),
-          (700, 130, 1152), (1000, 7, 126), (513, 1024, 640)]
+          (700, 130, 1152), (1000, 7, 126), (513, 1024, 640), (65, 64, 8192), (128, 130, 4100), (90, 201, 5000),
+          (24, 200, 8192), (48, 100, 4096), (16, 8200, 4224)]
 
 
 @pytest.mark.parametrize("dt", list(DT))
