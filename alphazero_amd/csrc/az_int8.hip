@@ -830,15 +830,16 @@ int az_i8_quantize_dev(int device, int dtype, int64_t rows, int64_t cols, const 
     if (!dtype_ok(dtype)) return refuse("az_i8_quantize: unknown dtype");
     if (rows < 0 || cols < 1 || n_src < 0 || ld_x < cols) return refuse("az_i8_quantize: bad shape or row distance");
     if (!index_dev && (taps != 1 || n_src != rows)) return refuse("az_i8_quantize: without an index taps is 1 and n_src is rows");
-    if (taps < 1 || cols > 0x7fffffff / taps || ld_x > (i64)1 << 40 || ld_q < taps * cols) return refuse("az_i8_quantize: bad taps or ld_q");
+    if (taps < 1 || cols > 0x7fffffff / taps || ld_x > (i64)1 << 40 || ld_q < taps * cols || ld_q > (i64)1 << 40)
+        return refuse("az_i8_quantize: bad taps or ld_q");
     if (rows == 0) {
         DeviceScope dev(device);
         return dev.rc;
     }
     if ((!x_dev && n_src > 0) || !q_dev || !scale_dev) return refuse("az_i8_quantize: null pointer");
     const i64 es = (i64)dtype_size(dtype);
-    const Span x = {x_dev, n_src, cols * es, ld_x * es}, q = {q_dev, rows, (i64)taps * cols, ld_q}, s = {scale_dev, 1, rows * 4, rows * 4};
-    const Span at = {index_dev, 1, rows * taps * 4, rows * taps * 4};
+    const Span x = {x_dev, n_src, cols * es, ld_x * es}, q = {q_dev, rows, (i64)taps * cols, ld_q}, s = {scale_dev, rows, 4, 4};
+    const Span at = {index_dev, rows, taps * (i64)4, taps * (i64)4};
     if (overlap(q, x) || overlap(q, s) || overlap(x, s) || overlap(q, at) || overlap(s, at))
         return refuse("az_i8_quantize: q and scale must not overlap an input or each other");
     DeviceScope dev(device);
@@ -851,7 +852,9 @@ static int mm_check(int64_t m, int64_t n, int64_t k, int64_t ld_x, int64_t ld_w,
     if (!dtype_ok(dtype)) return refuse("az_i8_matmul: unknown dtype");
     if (m < 0 || n < 0 || k < 1 || k > I8_MAX_K || m > 0x7fffffff || n > 0x7fffffff)
         return refuse("az_i8_matmul: bad shape (k is 1..131071)");
-    if (ld_x < k || ld_w < k || ld_y < n || (res && ld_res < n)) return refuse("az_i8_matmul: bad row distance");
+    const i64 most = (i64)1 << 40;
+    if (ld_x < k || ld_w < k || ld_y < n || (res && ld_res < n) || ld_x > most || ld_w > most || ld_y > most || (res && ld_res > most))
+        return refuse("az_i8_matmul: bad row distance");
     if (act < AZ_ACT_NONE || act > AZ_ACT_SILU) return refuse("az_i8_matmul: unknown activation");
     return AZ_OK;
 }

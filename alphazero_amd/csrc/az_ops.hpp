@@ -88,13 +88,19 @@ inline bool overlap(const void* p, size_t np, const void* q, size_t nq) {   // s
 struct Span {
     const void* p;
     i64 rows, width, ld;
+    size_t bytes() const {   // capped far above any memory
+        const i64 cap = (i64)1 << 56;
+        i64 n;
+        if (__builtin_mul_overflow(rows - 1, ld, &n) || __builtin_add_overflow(n, width, &n) || n > cap) n = cap;
+        return (size_t)n;
+    }
 };
 // whether two share a byte; columns of one buffer beside each other do not
 inline bool overlap(Span a, Span b) {
     if (!a.p || !b.p || a.rows < 1 || b.rows < 1) return false;
     if (a.rows == 1) a.ld = b.ld;
     if (b.rows == 1) b.ld = a.ld;
-    if (!overlap(a.p, (size_t)((a.rows - 1) * a.ld + a.width), b.p, (size_t)((b.rows - 1) * b.ld + b.width))) return false;
+    if (!overlap(a.p, a.bytes(), b.p, b.bytes())) return false;
     if (a.ld != b.ld || a.width > a.ld || b.width > b.ld) return true;
     const i64 off = (i64)((uintptr_t)b.p - (uintptr_t)a.p) % a.ld, d = off < 0 ? off + a.ld : off;   // b's first column in a's rows
     return d < a.width || d + b.width > a.ld;

@@ -58,6 +58,8 @@ def test_matmul_refuses():
         _refused(call(fn, ld_x=7), "row distance")
         _refused(call(fn, ld_w=7), "row distance")
         _refused(call(fn, ld_y=5), "row distance")
+        _refused(call(fn, ld_x=1 << 62), "row distance")
+        _refused(call(fn, ld_y=1 << 62), "row distance")
         _refused(call(fn, res=P, ld_res=5), "row distance")
         _refused(call(fn, act=3), "activation")
         _refused(call(fn, x=None), "null")
@@ -97,6 +99,8 @@ def test_int8_outputs_overlap_nothing():
     def quantize(x=0x1000, q=0x8000, s=0x9000, index=0xa000):
         return L.az_i8_quantize_dev(0, 0, 4, 8, C.c_void_p(x), 8, 5, C.c_void_p(index), 2, C.c_void_p(q), 16, C.c_void_p(s), None)
 
+    assert L.az_i8_quantize_dev(0, 0, 1 << 60, 8, C.c_void_p(0x10000), 1 << 40, 1 << 60, None, 1, C.c_void_p(0x1000), 8,
+                                C.c_void_p(0x9000), None) == ARG     # 2^100 bytes: counted without overflow
     for kw in (dict(q=0x1000), dict(q=0x1000 + 156), dict(s=0x1000), dict(s=0x8004), dict(index=0x8000), dict(index=0x9008)):
         _refused(quantize(**kw), "overlap")
     if _abi.device_count() == 0:
