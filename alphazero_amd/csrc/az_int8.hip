@@ -508,7 +508,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_mm_few(Mm p) {
     for (int f = 0; f < FM; f++) q[f] = p.q + (16 * f + row < p.m ? 16 * f + row : p.m - 1) * p.ld_q;
     i32x4 acc[FM] = {};
     const i64 whole = p.k & ~(i64)63;
-#pragma unroll 4
+    // a step at a time: more waves a CU hide the trips better than several steps' loads at once (us, one | 4 to 8: 42 x 128 x 1152 4.5 |
+    // 5.8, 1 x 8192 x 8192 12.5 | 13.1, 64 x 1024 x 1024 5.0 | 7.1)
     for (i64 k = wave * 64; k < whole; k += FEW_WAVES * 64) {
         i32x4 b, a[FM];
         __builtin_memcpy(&b, w + k + quarter * 16, 16);
@@ -604,7 +605,6 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void k_i8_linear_few(Mm p, const T*
         const i64 at = (wave + i * FEW_WAVES) * 64;
         if (at < whole) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*(const i32x4*)(q + at), b[i], acc, 0, 0, 0);
     }
-#pragma unroll 4
     for (i64 at = (wave + LIN_AHEAD * FEW_WAVES) * 64; at < whole; at += FEW_WAVES * 64) {
         i32x4 v;
         __builtin_memcpy(&v, w + at + quarter * 16, 16);
