@@ -73,6 +73,15 @@ __device__ inline void update_values(const Job& J, const Hyper& h, const i32 (&a
         if (!in[k]) v[k] = 0;
     }
 }
+// 2^14 / (norm + eps) as two factors to be multiplied one after the other.  The first is 1, or a power of two where the quotient
+// could leave float32's normal range: of an infinite factor even the zeros would become NaN.  Below 2^-150, half of the smallest
+// float32, the norm is 0 and so is every value; no factor needs to be larger for an eps that is.
+__device__ inline void norm_factors(double sum, double eps, float& first, float& second) {
+    double d = sqrt(sum) + eps;
+    if (d < 0x1p-150) d = 0x1p-150;   // a NaN stays one
+    first = d < 0x1p-100 ? 0x1p100f : d > 0x1p100 ? 0x1p-100f : 1.0f;
+    second = (float)(16384.0 / (d * first));
+}
 __device__ inline i64 split_off(i64 row, i64 rows, i64 k) { return ((k >> 4) * rows + row) * TILE_KB + (k & 15) * 2; }
 
 // eight values of a row from a multiple of eight on: their halves, 16 bytes each
@@ -145,7 +154,8 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if ((tid & 63) == 0) red[tid >> 6] = sum;
     __syncthreads();
-    const float scale = (float)(16384.0 / (sqrt((red[0] + red[1]) + (red[2] + red[3])) + h.eps));
+    float f1, f2;
+    norm_factors((red[0] + red[1]) + (red[2] + red[3]), h.eps, f1, f2);
     const bool flip = J.rows > J.cols;
     constexpr int U = 16;   // values a thread, all on their way at once
     float v[U];
@@ -162,7 +172,7 @@ __global__ __launch_bounds__(256) void k_ortho_init(Jobs js, Hyper h) {
 #pragma unroll
     for (int k = 0; k < U; k++) {
         const int e = tid + 256 * k, slow = e / OT, fast = e % OT;
-        tile[flip ? fast : slow][flip ? slow : fast] = v[k] * scale;
+        tile[flip ? fast : slow][flip ? slow : fast] = v[k] * f1 * f2;
     }
     __syncthreads();
     for (int u = tid; u < OT * OT / 8; u += 256) {   // pairs of lanes: 16 values of a row, 64 bytes
@@ -430,7 +440,8 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_init(Jobs js, Hyper h) {
     __syncthreads();
     sum = 0;
     for (int i = 0; i < NWAVES; i++) sum += red[i];
-    const float scale = (float)(16384.0 / (sqrt(sum) + h.eps));
+    float f1, f2;
+    norm_factors(sum, h.eps, f1, f2);
     f32x16 acc = {};
     for (int p = group * J.per_group; p < panels && p < (group + 1) * J.per_group; p++) {
         const int j0 = p * NPANEL;
@@ -452,7 +463,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_init(Jobs js, Hyper h) {
 #pragma unroll
             for (int k = 0; k < U; k++) {
                 const int e = e0 + NTHREADS * k, i = flip ? e % NARROW : e / NPANEL, j = flip ? e / NARROW : e % NPANEL;
-                if (i < height) nar_put(lds, i, j, v[k] * scale);
+                if (i < height) nar_put(lds, i, j, v[k] * f1 * f2);
             }
         }
         __syncthreads();
