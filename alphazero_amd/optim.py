@@ -20,7 +20,8 @@ def _coeffs(coeffs):
 
 def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, out=None):
     """The orthogonalisation of every matrix g[..., rows, cols] by `steps` Newton-Schulz products (float32-accurate):
-    X = G / (||G||_F + eps), X <- a X + (b A + c A^2) X with A = X X^T.  out: a contiguous tensor like g (may be g)."""
+    X = G / (||G||_F + eps), X <- a X + (b A + c A^2) X with A = X X^T.  out: a contiguous tensor like g (may be g).
+    Values of X are held to 2^-39 at best: of a matrix whose norm is 10^-4 of eps or less, fewer bits than float32's remain."""
     if g.dtype not in DTYPES or g.dim() < 2:
         raise AzError("orthogonalize: g must be float32, float16 or bfloat16 of at least two dimensions")
     no_grad("orthogonalize", g)

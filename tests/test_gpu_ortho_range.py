@@ -45,3 +45,17 @@ def test_an_eps_above_everything(rows, cols):
     from alphazero_amd import optim
     y = optim.orthogonalize(gradient(rows, cols, 3).cuda(), eps=1e300)
     assert (y == 0).all()
+
+
+@pytest.mark.parametrize("ratio", [1e2, 1e4, 1e6, 1e8])
+@pytest.mark.parametrize("rows,cols", SHAPES + [(128, 1152), (1024, 1024)])
+def test_an_eps_far_above_the_norm(rows, cols, ratio):
+    """X is small, and its low halves end at 2^-24 / 2^14: a value is off by up to 2^-39 however small it is.  The steps then only
+    multiply by a, and each adds as much again: (a^5 + a^4 + ...) 2^-39 <= a^5 / (1 - 1 / a) 2^-39 a value, beside the usual tolerance."""
+    from alphazero_amd import optim
+    g = gradient(rows, cols, 4)
+    eps = ratio * float(g.norm())
+    want, tol = allowed(g, torch.float32, eps=eps)
+    a = optim.COEFFS[0]
+    y = optim.orthogonalize(g.cuda(), eps=eps).cpu()
+    assert float((y.double() - want).norm()) <= tol + a ** 5 / (1 - 1 / a) * 2.0 ** -39 * (rows * cols) ** 0.5
