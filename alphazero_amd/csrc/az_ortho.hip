@@ -197,8 +197,12 @@ enum { GRAM = 0, POLY = 1, SQUARE = 2, STEP = 3, LAST = 4 };
 // Several steps at once.  A step on X costs 2.4 s^2 l multiplications and 0.8 s^3 (a symmetric product takes 0.8 of a whole one's
 // time).  Two or three can be made on the s x s side alone, A <- B A B and P <- B P, with X <- P X at their end: the default's five
 // steps cost 3.6 s^2 l + 11.2 s^3 as 2 + 3 against 9 s^2 l + 4 s^3 one by one, less from l = 1.33 s on.  All five at once would
-// not do: P's coefficients grow by (a^2)^k, and with them A's rounding; after two steps on X the small singular values have
-// grown by a^2 = 12 and 2 + 3 is as accurate as step by step (float32: 1.3e-6 to 4.1e-6 against 1.3e-6, 4.6e-5 for all five).
+// not do: P's coefficients grow by (a^2)^k, and with them A's rounding (4.6e-5 where step by step has 1.3e-6).  2 + 3 keeps A's rounding
+// from step to step too, where step by step makes A anew from X: that costs accuracy in float32, more or less by the matrix's singular
+// values (relative error, 2 + 3 | step by step | plain float32: 1024 x 1024 5.2e-6 | 2.2e-6 | 1.0e-6, 300 x 300 5.2e-6 | 1.3e-6 | 1.1e-6,
+// 512 x 2048 2.3e-6 | 2.2e-6 | 1.4e-6; six strong directions in noise, 512 x 4096 4.4e-6 | 2.0e-6 | 2.5e-6).  So results in float32 go step by
+// step, whatever the sizes; a result in 16 bits is rounded by up to 4.9e-4 (fp16) or 3.9e-3 of itself, a hundred times that, and takes
+// what is faster.
 
 // what a launch multiplies: s x s matrices 0..3 (a, b, c, d), and the power of two from its sums to what it stores
 struct Op {
@@ -873,10 +877,12 @@ static int run_jobs(Jobs& all, const Hyper& h, int steps, int dtype, hipStream_t
     AZ_DISPATCH_DTYPE(dtype, k_ortho_norm<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
     each_first(js, [](const Job& J) { return (i64)(J.sp / OT) * (J.lp / OT); });
     AZ_DISPATCH_DTYPE(dtype, k_ortho_init<T><<<dim3(js.first[js.n]), dim3(256), 0, st>>>(js, h));
-    // Steps on the s x s side where that should take less time.  A launch costs 5 us and its work at 0.9 PFLOP/s, or 0.1 us for
-    // every 16 values of the sums of its longest tile (both as measured, a symmetric product as 0.8 of a whole one).  2 + 3 | one by one,
-    // us: 2 x 333 x 1027 155 | 151, 2 x 400 x 800 158 | 147, 1024 x 1536 251 | 247, 1024 x 2048 264 | 273, 300 x 2000 151 | 167,
-    // 512 x 4096 211 | 272, 1024 x 4096 309 | 377
+    // Steps on the s x s side where the result has 16 bits (see above) and that should take less time for the list as a whole: launches
+    // are shared, and a second set of them for some of its matrices would cost more than it saves (1024 x 4096, 4096 x 1024 and two of
+    // 1024 x 1024, bf16: together 703 us, the squares step by step in launches of their own 833, all step by step 843).
+    // A launch costs 5 us and its work at 0.9 PFLOP/s, or 0.1 us for every 16 values of the sums of its longest tile (both as measured, a
+    // symmetric product as 0.8 of a whole one).  2 + 3 | one by one, us: 2 x 333 x 1027 155 | 151, 2 x 400 x 800 158 | 147, 1024 x 1536
+    // 251 | 247, 1024 x 2048 265 | 275, 300 x 2000 153 | 170, 512 x 4096 213 | 274, 1024 x 4096 323 | 394
     int len[16], n = 0, left = steps, squares = 0;
     while (left > 0) {
         len[n] = n == 0 ? (left < 2 ? left : 2) : (left < 3 ? left : 3);
@@ -893,7 +899,7 @@ static int run_jobs(Jobs& all, const Hyper& h, int steps, int dtype, hipStream_t
     }
     auto launch = [](double products, double k) { return 5.0 + fmax(6 * products / 0.9e9, 0.1 * k / 16); };
     const double on_x = launch(0.8 * s2l, longest_l) + launch(s2l, longest_s), on_a = launch(0.8 * s3, longest_s);
-    if (n * on_x + (steps + squares) * on_a > steps * (on_x + on_a) || steepest(h, steps) > 16.0)
+    if (dtype == AZ_F32 || n * on_x + (steps + squares) * on_a > steps * (on_x + on_a) || steepest(h, steps) > 16.0)
         for (n = 0; n < steps; n++) len[n] = 1;
     const Op gram = {0, 0, 0, 0x1p-16f};                                  // 2^14 2^14 -> 2^12
     auto poly = [](int out) { return Op{0, 0, out, 0x1p-24f}; };           // 2^12 2^12 -> 1, then 2^11
