@@ -279,7 +279,7 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
 #pragma unroll 2
         for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
             const int at = u % (2 * S::BM), r = at / 32 * 16 + at % 16, c = u / (2 * S::BM) * 16 + at / 16 % 2 * 8, m = m0 + r, n = n0 + c;
-            if (r >= mrows || c >= ncols) continue;
+            if (r >= mrows || c >= ncols || (SYM && n / OT > m / OT)) continue;
             float v[8];
             float* d = tile + r * PITCH + c;
             *(f32x4*)v = *(const f32x4*)d;
@@ -295,15 +295,16 @@ __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, 
             }
             split_store8(out + split_off(m, rows, n), v);
         }
-        // transposed: X for STEP, the mirrored tile for A and B.  The tiles across the diagonal cover both sides themselves: a
-        // mirrored value could differ from the computed one in its last bit, and both would be written.
-        if (SYM && n0 + S::BN > m0) return;
+        // transposed: X for STEP, the mirrored blocks for A and B.  Of the 64 x 64 blocks those on the diagonal cover both sides
+        // themselves (a mirrored value could differ from the computed one in its last bit, and both would be written); those above it
+        // are the ones below, mirrored.  So it is with tiles of either size, and a matrix's bits do not depend on which its list takes.
+        if (SYM && n0 + OT > m0 + S::BM - OT) return;
         if (MODE == POLY) __syncthreads();
         u8* outT = MODE == STEP ? J.x : out;
 #pragma unroll 2
         for (int u = tid; u < S::BM * S::BN / 8; u += S::THREADS) {
             const int c = u / 2 % S::BN, r = (u % 2 + u / (2 * S::BN) * 2) * 8;
-            if (r >= mrows || c >= ncols) continue;
+            if (r >= mrows || c >= ncols || (SYM && (n0 + c) / OT >= (m0 + r) / OT)) continue;
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] = tile[(r + e) * PITCH + c];

@@ -335,7 +335,7 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void *x_
  * 10^6: 8e-7, 1e-5, 1e-3).  out may be g itself.  steps 1..16, eps > 0.  Coefficients whose
  * iteration takes a singular value of [0, 1] above 2, or b A + c A^2 + a out of [-16, 16], are AZ_ERR_ARG (the halves' range).
  * A matrix that holds a NaN or an infinity comes out as NaN.  rows, cols <= 32768.
- * In float32 the steps are made one after the other.  Where the result has 16 bits several may be made at once, on the s x s products
+ * In float32 the steps are made one after the other, and a matrix comes out the same, bit for bit, beside any others.  Where the result has 16 bits several may be made at once, on the s x s products
  * alone, when that is faster for the matrices of the call together: a matrix's result can then differ in its last bits (float32
  * errors of up to 5e-6 instead of 2e-6, before the rounding) from the one it has alone. */
 size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols);

@@ -66,3 +66,37 @@ def test_float32_loses_nothing_to_the_order_of_its_steps(rows, cols, kind):
         one += relative(step_by_step(g.cuda()), want) / 8
         floats += relative(plain(g), want) / 8
     assert here <= 1.25 * max(one, floats), (here, one, floats)
+
+
+@pytest.mark.parametrize("dt,shapes", [
+    ("f32", [(27, 128, 20), (128, 1152, 3), (100, 2500, 5), (333, 1027, 17), (512, 512, 6), (300, 2000, 7), (640, 1500, 3), (200, 200, 40)]),
+    ("f16", [(27, 128, 20), (128, 1152, 3), (100, 2500, 5)]), ("bf16", [(27, 128, 20), (128, 1152, 3), (100, 2500, 5)])])
+def test_a_matrix_does_not_depend_on_its_batch(dt, shapes):
+    """the same bits alone and in a batch, which takes tiles of the other size"""
+    from alphazero_amd import optim
+    for rows, cols, n in shapes:
+        g = torch.stack([gradient(rows, cols, i) for i in range(n)]).to(DT[dt]).cuda()
+        y = optim.orthogonalize(g)
+        for i in (0, n // 2, n - 1):
+            assert torch.equal(optim.orthogonalize(g[i]), y[i]), (rows, cols, i)
+
+
+def test_a_weight_does_not_depend_on_its_companions():
+    """a float32 update of matrices of all forms in one call, in another order, and one by one"""
+    from alphazero_amd import optim
+    shapes = [(300, 300), (1500, 300), (128, 128), (128, 27), (512, 512), (100, 2500), (64, 576), (256, 1100), (700, 640), (20, 9),
+              (1024, 300), (130, 130), (128, 1152), (2100, 64), (900, 1000), (150, 150), (150, 160), (260, 1500)]
+
+    def fresh():
+        return [(gradient(*s, 50 + i, scale=0.1).cuda(), gradient(*s, i).cuda(), gradient(*s, 100 + i).cuda()) for i, s in enumerate(shapes)]
+
+    together, turned, alone = fresh(), fresh(), fresh()
+    order = list(range(len(shapes)))[::-1]
+    for _ in range(2):
+        optim.muon_step([t[0] for t in together], [t[1] for t in together], [t[2] for t in together], lr=0.02)
+        optim.muon_step([turned[i][0] for i in order], [turned[i][1] for i in order], [turned[i][2] for i in order], lr=0.02)
+        for w, g, m in alone:
+            optim.muon_step([w], [g], [m], lr=0.02)
+    for s, a, b, c in zip(shapes, together, turned, alone):
+        for k in (0, 2):
+            assert torch.equal(a[k], b[k]) and torch.equal(a[k], c[k]), s
