@@ -343,13 +343,15 @@ using OTile64 = TileShape<64, 64, 2, 2, 3, 4>;   // few tiles: what counts is th
 // launch adds up the panels' parts of A = X X^T (in order, so the sum is the same every time); in the second every workgroup owns
 // some panels and
 //   1. takes A into LDS,
-//   2. makes B = a I + b A + c A A^T for itself, and as a rule the next step's as well, of B A B (two steps a launch),
+//   2. makes B = a I + b A + c A A^T for itself, and where the result has 16 bits the next step's as well, of B A B (two steps a launch),
 //   3. multiplies its panels by it, keeping T for the next launch, and adds up their part of the next Gram matrix.
 // What bounds it is latency: 5 steps of a 128 x 1152 matrix are 0.4 GFLOP, but 15 products one after the other; between launches,
-// each product would start on cold operands.  Seven matrices up to 128 x 1152 in one call: norm 6 us, init 12, sums 4.5 a launch, two
-// steps 24 (2.5 for each of the four products more, which read 512 KB of LDS; one step is 14.8), the last alone 12: 89 us in all, 104 with
-// one step a launch (us, this form | the wide matrices': 89 | 136; alone, 128 x 1152 81 | 104, 128 x 32768 173 | 483, 4 x 100 x 5000
-// 108 | 181, 16 x 64 x 64 50 | 77, 128 x 128 80 | 76).
+// each product would start on cold operands.  Seven float32 matrices up to 128 x 1152 in one call: norm 6 us, init 12, sums 4.5 a
+// launch, a step 15, the last 12: 105 us in all.  Two steps a launch take 24 us (2.5 for each of the four products more, which read 512 KB
+// of LDS); 16-bit results are made so (us, two steps a launch | one: 128 x 1152 83 | 98, 128 x 32768 174 | 233, 4 x 100 x 5000 107 |
+// 136, 16 x 64 x 64 54 | 74), float32 ones are not: the second step's A keeps the first one's rounding (relative error, two | one | plain
+// float32: 32 x 32 1.5e-6 | 0.7e-6 | 0.8e-6, 128 x 128 1.4e-6 | 0.8e-6 | 1.3e-6, 128 x 1152 1.15e-6 | 1.14e-6 | 1.43e-6).  The wide matrices'
+// launches instead of these: the seven 136 us, 128 x 128 76.
 //
 // T goes through memory in the order in which the MFMA of 3. takes it and the one before leaves it.  D = B T^T leaves lane
 // (h = lane / 32, j = lane % 32) rows i = 8 (r / 4) + 4 h + r % 4 of column j: eight registers are eight values of k for lane (h, j) of the
@@ -840,7 +842,7 @@ static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_
     const dim3 grid(most, js.n), block(NTHREADS);
     AZ_DISPATCH_DTYPE(dtype, k_narrow_init<T><<<grid, block, NBUF, st>>>(js, h));
     const dim3 grid_sum(10, js.n);   // blocks of a 128 x 128 matrix's lower triangle
-    const bool pairs = steepest(h, steps) <= 16.0;
+    const bool pairs = dtype != AZ_F32 && steepest(h, steps) <= 16.0;
     int cur = 0;
     for (int done = 0; done < steps; cur ^= 1) {
         const bool two = pairs && done + 2 <= steps;

@@ -47,11 +47,12 @@ def strong(rows, cols, seed):
 
 
 # squares and rectangles, short and long ones
+NARROW = [(16, 16), (32, 32), (64, 64), (128, 128), (27, 128), (128, 27), (128, 256), (128, 1152), (64, 1100), (1100, 64), (32, 4096), (128, 2100)]
 WIDE = [(300, 300), (200, 300), (512, 512), (300, 600), (600, 300), (300, 1250), (300, 2000), (256, 2048)]
 
 
 @pytest.mark.parametrize("kind", [gradient, strong])
-@pytest.mark.parametrize("rows,cols", WIDE)
+@pytest.mark.parametrize("rows,cols", NARROW + WIDE)
 def test_float32_loses_nothing_to_the_order_of_its_steps(rows, cols, kind):
     """However the steps are grouped: the mean error over seeds is at most a quarter above that of steps one by one on the same
     operands and sums, or of a plain float32 evaluation, if that is larger.  (The error varies by less than a quarter from seed to
