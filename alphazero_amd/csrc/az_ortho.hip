@@ -842,7 +842,7 @@ static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_
     const dim3 grid(most, js.n), block(NTHREADS);
     AZ_DISPATCH_DTYPE(dtype, k_narrow_init<T><<<grid, block, NBUF, st>>>(js, h));
     const dim3 grid_sum(10, js.n);   // blocks of a 128 x 128 matrix's lower triangle
-    const bool pairs = dtype != AZ_F32 && steepest(h, steps) <= 16.0;
+    const bool pairs = dtype != AZ_F32 && steepest(h, steps) <= 16.0;   // (see above)
     int cur = 0;
     for (int done = 0; done < steps; cur ^= 1) {
         const bool two = pairs && done + 2 <= steps;
@@ -852,7 +852,8 @@ static int run_narrow(Jobs& js, const Hyper& h, int steps, int dtype, hipStream_
         const Narrow pass = {ldexpf(1.0f, e - 22), ldexpf(1.0f, last ? -14 - e : -e)};
         k_narrow_sum<<<grid_sum, dim3(256), 0, st>>>(js);
         if (last && two) {
-            AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true, true><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass));
+            if (dtype == AZ_F16) k_narrow_step<f16, true, true><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass);
+            else k_narrow_step<bf16, true, true><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass);
         } else if (last) {
             AZ_DISPATCH_DTYPE(dtype, k_narrow_step<T, true, false><<<grid, block, NSTEP_LDS, st>>>(js, h, cur, pass));
         } else if (two) {
