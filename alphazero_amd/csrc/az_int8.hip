@@ -371,7 +371,8 @@ __device__ inline void put(const Mm& p, i64 m, i64 n, int sum, float scale) {
 // 1.66 GHz (power): a k slice costs as many LDS cycles as MFMA cycles.  86016 x 128 x 1152, 128 x 128 tiles: 29 us, 4.2 TB/s of rows
 // read and results written, SiLU on the way.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 7.8 us, one after the other:
 // launch, first tiles, 17 steps, residual, stores.
-template <class T, class S>
+// RES: with a residual, whose values take registers (128 x 128 tile: 96, 70 without: three workgroups a CU).
+template <class T, class S, bool RES>
 __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u32 tiles_n, u32 steps_per_split, int* part) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -434,7 +435,7 @@ __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u3
 #pragma unroll
             for (int i = 0; i < S::FM; i++) {
                 float res[16][W];
-                if (p.res) {   // a block's residuals on their way at once
+                if constexpr (RES) {   // a block's residuals on their way at once
                     T raw[16][W];
 #pragma unroll
                     for (int r = 0; r < 16; r++) {
@@ -709,7 +710,9 @@ template <class T, class S>
 static int launch_tile(const Mm& p, const MmPlan& P, int* part, hipStream_t st) {
     const i64 tm = (p.m + S::BM - 1) / S::BM, tn = (p.n + S::BN - 1) / S::BN;
     if (tm * tn > 0x7fffffff) return refuse("az_i8_matmul: more than 2^31 tiles");
-    k_i8_mm_tile<T, S><<<dim3((u32)(tm * tn), P.splits), dim3(S::THREADS), S::LDS, st>>>(p, (u32)tm, (u32)tn, P.steps_per_split, part);
+    const dim3 grid((u32)(tm * tn), P.splits), block(S::THREADS);
+    if (p.res && !part) k_i8_mm_tile<T, S, true><<<grid, block, S::LDS, st>>>(p, (u32)tm, (u32)tn, P.steps_per_split, part);
+    else k_i8_mm_tile<T, S, false><<<grid, block, S::LDS, st>>>(p, (u32)tm, (u32)tn, P.steps_per_split, part);
     if (part) {
         const i64 blocks = (p.m * p.n + 255) / 256;
         k_i8_join<T><<<dim3((u32)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, st>>>(p, P.splits, part);
