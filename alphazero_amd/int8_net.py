@@ -7,6 +7,7 @@ An object of this class is a policy_value_fn: MCTS_AZ / AlphaZeroPlayer call its
 Each weight is off by at most half of 1/127 of its channel's largest, each activation by half of 1/127 of its row's.
 """
 import re
+import threading
 
 import numpy as np
 import torch
@@ -15,6 +16,17 @@ from . import int8
 from ._abi import AzError
 
 BN_EPS = 1e-5   # torch.nn.BatchNorm2d's
+LOCK = threading.RLock()   # held while a network's tensors on the device change
+
+
+def capturing(device):
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def settle(device):
+    """what was launched on the current stream is done: any stream may read it from now on"""
+    torch.cuda.current_stream(device).synchronize()
 
 
 def neighbour_index(rows, cols, boards, device):
@@ -33,15 +45,20 @@ def neighbour_index(rows, cols, boards, device):
 class Int8CNN:
     def __init__(self, state_dict, board=(6, 7), device="cuda", dtype=torch.float32, game="Connect4"):
         """state_dict: of the reference's CNN (or a module that has one).  dtype: of the activations between layers; float32
-        holds whatever a checkpoint does, float16 halves their traffic for networks whose activations stay below 65504."""
+        holds whatever a checkpoint does, float16 halves their traffic for networks whose activations stay below 65504.
+
+        Threads and streams may share an object.  forward_device may be captured into a graph once it has been called with as
+        many boards or more; the graph needs the object alive."""
         if dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise AzError("Int8CNN: dtype must be float32, float16 or bfloat16")
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise AzError("Int8CNN runs on the GPU only (no CPU path)")
+        if self.device.index is None:      # this one, whichever is current at a call
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.board, self.dtype, self.game = (int(board[0]), int(board[1])), dtype, game
         self.cells = self.board[0] * self.board[1]
-        self._index = {}
+        self._tables = ()
         self.load_state_dict(state_dict.state_dict() if hasattr(state_dict, "state_dict") else state_dict)
 
     def name(self):
@@ -106,11 +123,22 @@ class Int8CNN:
 
     # ---- inference
     def _neighbours(self, boards):
-        if boards not in self._index:
-            if len(self._index) >= 8:      # a search asks for a handful of batch sizes
-                self._index.clear()
-            self._index[boards] = neighbour_index(*self.board, boards, self.device)
-        return self._index[boards]
+        """The first rows of a larger batch's table are a smaller one's.  Tables hold a power of two of boards; they are complete before
+        any call sees them and live as long as the object, so that no stream, thread or captured graph is left with one that changes:
+        at most twice the memory of the largest, 1.5 KB a board of 42 cells."""
+        rows = boards * self.cells
+        for t in self._tables:
+            if t.shape[0] >= rows:
+                return t[:rows]
+        with LOCK:
+            if self._tables and self._tables[-1].shape[0] >= rows:
+                return self._tables[-1][:rows]
+            if capturing(self.device):
+                raise AzError("Int8CNN: call with %d boards once before capturing a graph of it" % boards)
+            t = neighbour_index(*self.board, max(64, 1 << (boards - 1).bit_length()), self.device)
+            settle(self.device)
+            self._tables += (t,)
+        return t[:rows]
 
     def _conv3(self, x, name, boards):
         q, s = int8.quantize_rows(x, index=self._neighbours(boards))
@@ -164,7 +192,7 @@ class Int8CNN:
     def net_forward(self, states):
         """SelfPlayEngine.net_forward's form, of packed positions: (logp, logv, probs, value)"""
         from .engine import env_planes_batch
-        planes = torch.from_numpy(env_planes_batch(self.game, states, device=self.device.index or 0))
+        planes = torch.from_numpy(env_planes_batch(self.game, states, device=self.device.index))
         p, v = self.forward_device(planes)
         logp, logv = torch.log_softmax(p, 1), torch.log_softmax(v, 1)
         w = logv.exp()

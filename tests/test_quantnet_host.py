@@ -1,0 +1,99 @@
+"""Int8CNN's bookkeeping and layout on the CPU: what it keeps on the device, with float forms in the place of the 8-bit calls."""
+import sys
+import threading
+
+import pytest
+import torch
+
+from alphazero_amd import int8, int8_net
+from alphazero_amd._abi import AzError
+from alphazero_amd.int8_net import Int8CNN, neighbour_index
+from test_gpu_quantnet import Net, jitter, positions
+
+
+@pytest.fixture
+def on_the_cpu(monkeypatch):
+    """Int8CNN on the CPU in float64; says whether a stream is being captured as told"""
+    said = {"capturing": False, "settled": 0}
+
+    def settle(device):
+        said["settled"] += 1
+
+    def quantize_rows(x, index=None):
+        rows = x.double()
+        if index is not None:
+            rows = torch.cat((rows, rows.new_zeros(1, x.shape[1])))[index.long()].reshape(index.shape[0], -1)
+        return rows, torch.ones(rows.shape[0], dtype=torch.float64)
+
+    def matmul(q, scale, w, w_scale, bias=None, residual=None, act="none", dtype=None, out=None):
+        y = q @ w.t() + bias
+        y = y if residual is None else y + residual
+        return torch.nn.functional.silu(y) if act == "silu" else y
+
+    monkeypatch.setattr(int8_net, "capturing", lambda device: said["capturing"])
+    monkeypatch.setattr(int8_net, "settle", settle)
+    monkeypatch.setattr(int8, "quantize_rows", quantize_rows)
+    monkeypatch.setattr(int8, "matmul", matmul)
+    monkeypatch.setattr(int8, "linear", lambda x, w, ws, **kw: matmul(x.double(), None, w, ws, **kw))
+
+    def make(net=None, board=(6, 7)):
+        q = Int8CNN.__new__(Int8CNN)
+        q.device, q.board, q.dtype, q.game, q.cells = torch.device("cpu"), board, torch.float64, "Connect4", board[0] * board[1]
+        q._tables = ()
+        if net is not None:
+            q.load_state_dict(net.state_dict())
+        return q
+
+    return make, said
+
+
+def test_a_table_that_was_handed_out_stays_what_it_is(on_the_cpu):
+    """a captured graph and other streams hold its address"""
+    make, said = on_the_cpu
+    q = make()
+    held = {b: q._neighbours(b) for b in (5, 64, 1, 65, 300)}
+    places = {b: t.data_ptr() for b, t in held.items()}
+    for b in range(1, 700, 13):
+        assert torch.equal(q._neighbours(b), neighbour_index(6, 7, b, "cpu"))
+    for b, t in held.items():
+        assert q._neighbours(b).data_ptr() == places[b] and torch.equal(t, neighbour_index(6, 7, b, "cpu"))
+    assert said["settled"] == len(q._tables) == 4           # of 64, 128, 512 and 1024 boards
+    assert sum(t.shape[0] for t in q._tables) <= 2 * q._tables[-1].shape[0]
+
+
+def test_a_table_is_not_made_inside_a_capture(on_the_cpu):
+    make, said = on_the_cpu
+    q = make()
+    q._neighbours(64)
+    said["capturing"] = True
+    assert q._neighbours(3).shape == (126, 9)
+    with pytest.raises(AzError, match="65 boards once before"):
+        q._neighbours(65)
+    assert len(q._tables) == 1
+
+
+def test_threads_that_ask_for_many_batch_sizes(on_the_cpu):
+    make, _ = on_the_cpu
+    q = make(board=(3, 3))
+    bad = []
+
+    def ask(k):
+        try:
+            for i in range(400):
+                b = 1 + (i * 37 + k * 211) % 900
+                if q._neighbours(b).shape != (9 * b, 9):
+                    bad.append(b)
+        except Exception as e:
+            bad.append(repr(e))
+
+    interval = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    try:
+        threads = [threading.Thread(target=ask, args=(k,)) for k in range(4)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(interval)
+    assert bad == []
