@@ -24,6 +24,11 @@ def capturing(device):
         return torch.cuda.is_current_stream_capturing()
 
 
+def idle(device):
+    """everything that was launched on the device is done"""
+    torch.cuda.synchronize(device)
+
+
 def settle(device):
     """what was launched on the current stream is done: any stream may read it from now on"""
     torch.cuda.current_stream(device).synchronize()
@@ -48,7 +53,7 @@ class Int8CNN:
         holds whatever a checkpoint does, float16 halves their traffic for networks whose activations stay below 65504.
 
         Threads and streams may share an object.  forward_device may be captured into a graph once it has been called with as
-        many boards or more; the graph needs the object alive."""
+        many boards or more; the graph needs the object alive, and goes on with the weights that are loaded later."""
         if dtype not in (torch.float32, torch.float16, torch.bfloat16):
             raise AzError("Int8CNN: dtype must be float32, float16 or bfloat16")
         self.device = torch.device(device)
@@ -58,7 +63,7 @@ class Int8CNN:
             self.device = torch.device("cuda", torch.cuda.current_device())
         self.board, self.dtype, self.game = (int(board[0]), int(board[1])), dtype, game
         self.cells = self.board[0] * self.board[1]
-        self._tables = ()
+        self._tables, self.layers, self._captured = (), {}, False
         self.load_state_dict(state_dict.state_dict() if hasattr(state_dict, "state_dict") else state_dict)
 
     def name(self):
@@ -73,8 +78,31 @@ class Int8CNN:
 
     # ---- weights
     def load_state_dict(self, sd):
-        layers = self._read(sd)
-        self.layers = {k: self._quantize(*v) for k, v in layers.items()}     # only when all of it was accepted
+        """All of it or nothing.  Weights of the shapes that are there go into the same memory, after everything that was launched on the
+        device before: no call computes with some of either, and a captured graph goes on with the new ones."""
+        with torch.inference_mode(False), torch.no_grad():
+            if capturing(self.device):
+                raise AzError("Int8CNN: weights cannot be loaded while a graph is captured")
+            layers = self._read(sd)
+            new = {k: self._quantize(*v) for k, v in layers.items()}
+            settle(self.device)
+            with LOCK:
+                old = self.layers
+                alike = old.keys() == new.keys() and all(a.shape == b.shape for k in new for a, b in zip(old[k], new[k]))
+                if old and not alike and self._captured:
+                    raise AzError("Int8CNN: weights of other shapes than the captured graph's: make a new Int8CNN for them")
+                if old:
+                    idle(self.device)
+                if alike:
+                    for k in new:
+                        for a, b in zip(old[k], new[k]):
+                            a.copy_(b)
+                    settle(self.device)
+                else:
+                    self.layers = new
+                self.n_blocks = sum(k.startswith("mix") for k in new)
+                self.h_dim, self.in_dim = sd["hidden.0.weight"].shape[:2]
+                self.n_actions = new["policy_out"][0].shape[0]
 
     def sync_from(self, module):
         """the hot reload after a training step: module is the reference's torch CNN (or anything with state_dict())"""
@@ -111,10 +139,6 @@ class Int8CNN:
                 raise AzError("Int8CNN: %s_head.4 takes %d values, the board gives %d" % (head, w.shape[1], c * self.cells))
             w = w.view(-1, c, self.cells).permute(0, 2, 1).reshape(w.shape[0], -1)  # nn.Flatten's (channel, cell) -> (cell, channel)
             out[head + "_out"] = (w, get(head + "_head.4.bias"))
-        self.n_blocks = len(blocks)
-        self.in_dim = sd["hidden.0.weight"].shape[1]
-        self.h_dim = sd["hidden.0.weight"].shape[0]
-        self.n_actions = out["policy_out"][0].shape[0]
         return out
 
     def _quantize(self, w, b):
@@ -155,18 +179,20 @@ class Int8CNN:
     @torch.no_grad()
     def forward_device(self, planes):
         """(logits [B, n_actions], value logits [B, 3]) float32 of planes [B, in_dim, rows, cols], all on the device"""
-        if planes.dim() != 4 or tuple(planes.shape[1:]) != (self.in_dim,) + self.board:
-            raise AzError("Int8CNN: planes must be [B, %d, %d, %d]" % ((self.in_dim,) + self.board))
-        B = planes.shape[0]
-        if B == 0:
-            return (torch.empty(0, self.n_actions, device=self.device), torch.empty(0, self.layers["value_out"][0].shape[0], device=self.device))
-        x = planes.to(self.device, self.dtype).permute(0, 2, 3, 1).reshape(B * self.cells, self.in_dim).contiguous()
-        x = self._conv3(x, "stem", B)
-        for i in range(self.n_blocks):
-            t = self._conv3(x, "conv%d" % i, B)
-            w, ws, b = self.layers["mix%d" % i]
-            x = int8.linear(t, w, ws, bias=b, residual=x, act="silu")
-        return self._logits(x, "policy", B), self._logits(x, "value", B)
+        with LOCK:      # a reload waits until all of a call has been launched
+            if planes.dim() != 4 or tuple(planes.shape[1:]) != (self.in_dim,) + self.board:
+                raise AzError("Int8CNN: planes must be [B, %d, %d, %d]" % ((self.in_dim,) + self.board))
+            B = planes.shape[0]
+            if B == 0:
+                return (torch.empty(0, self.n_actions, device=self.device), torch.empty(0, self.layers["value_out"][0].shape[0], device=self.device))
+            self._captured = self._captured or capturing(self.device)
+            x = planes.to(self.device, self.dtype).permute(0, 2, 3, 1).reshape(B * self.cells, self.in_dim).contiguous()
+            x = self._conv3(x, "stem", B)
+            for i in range(self.n_blocks):
+                t = self._conv3(x, "conv%d" % i, B)
+                w, ws, b = self.layers["mix%d" % i]
+                x = int8.linear(t, w, ws, bias=b, residual=x, act="silu")
+            return self._logits(x, "policy", B), self._logits(x, "value", B)
 
     def forward(self, state):
         """(log_prob (B, n_actions), value_log_prob (B, 3)) float32 numpy -- Network.py:60-64"""

@@ -109,3 +109,69 @@ def test_a_batch_that_has_no_table_yet_is_refused_inside_a_capture():
     torch.cuda.synchronize()
     assert len(said) == 1 and "once before" in said[0] and torch.equal(out, s * 2)
     assert same(q.forward_device(s), make().forward_device(s))
+
+
+def test_a_graph_goes_on_with_reloaded_weights():
+    from alphazero_amd._abi import AzError
+    q = make()
+    s = positions(33, 1).cuda()
+    q.forward_device(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = q.forward_device(s)
+    for seed in (3, 4, 5, 6, 7):
+        q.sync_from(net(seed=seed))
+        filler = torch.full((4 << 20,), 77, dtype=torch.int8, device="cuda")       # takes what was freed, if anything was
+        s.copy_(positions(33, seed))
+        for _ in range(2):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert same(out, make(seed=seed).forward_device(s)) and same(out, q.forward_device(s)) and filler.numel()
+    with pytest.raises(AzError, match="other shapes"):
+        q.sync_from(net(h=32))
+
+
+def test_a_reload_waits_for_the_calls_before_it():
+    q, s = make(seed=3), positions(500, 2).cuda()
+    old, new = make(seed=3).forward_device(s), make(seed=4).forward_device(s)
+    q.forward_device(s)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        kept = busy()
+        a = q.forward_device(s)
+    q.sync_from(net(seed=4))
+    b = q.forward_device(s)
+    torch.cuda.synchronize()
+    assert same(a, old) and same(b, new) and not same(old, new) and kept.shape == (4096, 4096)
+
+
+def test_reloads_between_the_calls_of_other_threads():
+    """every answer is the one of some accepted weights as a whole"""
+    q, s = make(h=32, seed=3), positions(70, 2).cuda()
+    allowed = [make(h=32, seed=i).forward_device(s) for i in (3, 4)]
+    states = [net(h=32, seed=i).state_dict() for i in (3, 4)]
+    q.forward_device(s)
+    torch.cuda.synchronize()
+    bad, done = [], threading.Event()
+
+    def ask():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                while not done.is_set():
+                    y = q.forward_device(s)
+                    torch.cuda.current_stream().synchronize()
+                    if not any(same(y, w) for w in allowed):
+                        bad.append(y)
+        except Exception as e:
+            bad.append(repr(e))
+
+    threads = [threading.Thread(target=ask) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for i in range(20):
+        q.load_state_dict(states[(i + 1) % 2])
+    done.set()
+    for t in threads:
+        t.join()
+    assert bad == []

@@ -14,10 +14,13 @@ from test_gpu_quantnet import Net, jitter, positions
 @pytest.fixture
 def on_the_cpu(monkeypatch):
     """Int8CNN on the CPU in float64; says whether a stream is being captured as told"""
-    said = {"capturing": False, "settled": 0}
+    said = {"capturing": False, "settled": 0, "idle": 0}
 
     def settle(device):
         said["settled"] += 1
+
+    def idle(device):
+        said["idle"] += 1
 
     def quantize_rows(x, index=None):
         rows = x.double()
@@ -32,6 +35,7 @@ def on_the_cpu(monkeypatch):
 
     monkeypatch.setattr(int8_net, "capturing", lambda device: said["capturing"])
     monkeypatch.setattr(int8_net, "settle", settle)
+    monkeypatch.setattr(int8_net, "idle", idle)
     monkeypatch.setattr(int8, "quantize_rows", quantize_rows)
     monkeypatch.setattr(int8, "matmul", matmul)
     monkeypatch.setattr(int8, "linear", lambda x, w, ws, **kw: matmul(x.double(), None, w, ws, **kw))
@@ -39,7 +43,7 @@ def on_the_cpu(monkeypatch):
     def make(net=None, board=(6, 7)):
         q = Int8CNN.__new__(Int8CNN)
         q.device, q.board, q.dtype, q.game, q.cells = torch.device("cpu"), board, torch.float64, "Connect4", board[0] * board[1]
-        q._tables = ()
+        q._tables, q.layers, q._captured = (), {}, False
         if net is not None:
             q.load_state_dict(net.state_dict())
         return q
@@ -97,3 +101,55 @@ def test_threads_that_ask_for_many_batch_sizes(on_the_cpu):
     finally:
         sys.setswitchinterval(interval)
     assert bad == []
+
+
+def layers_of(q):
+    return {k: [t.clone() for t in v] for k, v in q.layers.items()}
+
+
+def same_layers(a, b):
+    return a.keys() == b.keys() and all(torch.equal(x, y) for k in a for x, y in zip(a[k], b[k]))
+
+
+def test_a_reload_goes_into_the_same_memory(on_the_cpu):
+    """a captured graph and calls on other streams hold its address"""
+    make, said = on_the_cpu
+    q = make(jitter(Net(h=16), 1))
+    places = {k: [t.data_ptr() for t in v] for k, v in q.layers.items()}
+    other = jitter(Net(h=16), 2)
+    before = said["idle"]
+    q.sync_from(other)
+    assert said["idle"] == before + 1                      # what was launched before has read the old ones
+    assert {k: [t.data_ptr() for t in v] for k, v in q.layers.items()} == places
+    assert same_layers(q.layers, make(other).layers)
+
+
+def test_a_reload_beside_a_capture(on_the_cpu):
+    make, said = on_the_cpu
+    net = jitter(Net(h=16), 1)
+    q = make(net)
+    s = positions(3, 1)
+    q.forward_device(s)
+    kept, want = layers_of(q), q.forward_device(s)
+    said["capturing"] = True
+    with pytest.raises(AzError, match="while a graph is captured"):
+        q.sync_from(jitter(Net(h=16), 2))
+    q.forward_device(s)
+    said["capturing"] = False
+    with pytest.raises(AzError, match="other shapes"):
+        q.sync_from(jitter(Net(h=24), 2))                  # the graph reads the old ones
+    assert same_layers(q.layers, kept) and (q.h_dim, q.in_dim, q.n_blocks, q.n_actions) == (16, 3, 3, 7)
+    assert all(torch.equal(a, b) for a, b in zip(q.forward_device(s), want))
+    free = make(net)
+    free.sync_from(jitter(Net(in_dim=4, h=24, out_dim=9), 2))
+    assert (free.h_dim, free.in_dim, free.n_actions) == (24, 4, 9)
+    assert free.forward_device(positions(3, 1, in_dim=4))[0].shape == (3, 9)
+
+
+def test_weights_loaded_in_inference_mode_can_be_reloaded_outside(on_the_cpu):
+    make, _ = on_the_cpu
+    with torch.inference_mode():
+        q = make(jitter(Net(h=16), 1))
+    other = jitter(Net(h=16), 2)
+    q.sync_from(other)
+    assert same_layers(q.layers, make(other).layers)
