@@ -127,18 +127,30 @@ class Int8CNN:
             w = w * k.view(-1, 1, 1, 1)
             return w.permute(0, 2, 3, 1).reshape(w.shape[0], -1), b - mean * k      # (tap, input channel)
 
+        def fits(name, inputs, taps, outputs=None):
+            w, bias = out[name]
+            if w.shape[1] != inputs * taps or (outputs is not None and w.shape[0] != outputs) or bias.shape != (w.shape[0],):
+                raise AzError("Int8CNN: %s does not fit the layers around it" % name)
+            if not (torch.isfinite(w.float()).all() and torch.isfinite(bias.float()).all()):
+                raise AzError("Int8CNN: %s is not finite in float32 once its BatchNorm is folded in" % name)
+            return w.shape[0]
+
         out = {"stem": folded("hidden.0", "hidden.1")}
+        h = fits("stem", get("hidden.0.weight").shape[1], 9)
         blocks = sorted({int(m.group(1)) for m in (re.match(r"hidden\.(\d+)\.conv\.0\.weight$", k) for k in sd) if m})
         for i, b in enumerate(blocks):
             out["conv%d" % i] = folded("hidden.%d.conv.0" % b, "hidden.%d.conv.1" % b)
             out["mix%d" % i] = folded("hidden.%d.conv.4" % b, "hidden.%d.conv.5" % b)
-        for head in ("policy", "value"):
+            fits("mix%d" % i, fits("conv%d" % i, h, 9), 1, h)
+        for head, classes in (("policy", None), ("value", 3)):
             out[head + "_conv"] = folded(head + "_head.0", head + "_head.1")
-            w, c = get(head + "_head.4.weight"), out[head + "_conv"][0].shape[0]
-            if w.shape[1] != c * self.cells:
-                raise AzError("Int8CNN: %s_head.4 takes %d values, the board gives %d" % (head, w.shape[1], c * self.cells))
+            c = fits(head + "_conv", h, 1)
+            w = get(head + "_head.4.weight")
+            if w.dim() != 2 or w.shape[1] != c * self.cells:
+                raise AzError("Int8CNN: %s_head.4 takes %d values, the board gives %d" % (head, w.shape[-1], c * self.cells))
             w = w.view(-1, c, self.cells).permute(0, 2, 1).reshape(w.shape[0], -1)  # nn.Flatten's (channel, cell) -> (cell, channel)
             out[head + "_out"] = (w, get(head + "_head.4.bias"))
+            fits(head + "_out", c * self.cells, 1, classes)
         return out
 
     def _quantize(self, w, b):

@@ -153,3 +153,30 @@ def test_weights_loaded_in_inference_mode_can_be_reloaded_outside(on_the_cpu):
     other = jitter(Net(h=16), 2)
     q.sync_from(other)
     assert same_layers(q.layers, make(other).layers)
+
+
+def test_what_cannot_be_evaluated_is_refused_whole(on_the_cpu):
+    make, _ = on_the_cpu
+    q = make(jitter(Net(h=16), 1))
+    kept = layers_of(q)
+    good = jitter(Net(h=16), 2).state_dict()
+    conv, conv1, bn = torch.nn.Conv2d(16, 16, 3).weight.data, torch.nn.Conv2d(16, 16, 1).weight.data, good["hidden.5.conv.1.running_var"]
+    for key, value in [("hidden.5.conv.0.weight", conv1), ("hidden.5.conv.4.weight", conv), ("hidden.0.weight", conv1[:, :3]),
+                       ("hidden.5.conv.0.weight", conv[:, :8]), ("hidden.5.conv.4.weight", conv1[:8]), ("policy_head.0.weight", conv[:3]),
+                       ("policy_head.0.weight", conv1[:2]), ("value_head.4.weight", good["value_head.4.weight"][:2]),
+                       ("value_head.4.bias", torch.zeros(2)), ("policy_head.4.bias", torch.zeros(6)),
+                       ("hidden.5.conv.1.running_var", torch.full_like(bn, -1.0)),                    # the fold's root of a negative
+                       ("hidden.5.conv.1.weight", torch.full(bn.shape, 1e42, dtype=torch.float64))]:      # above float32
+        bad = dict(good)
+        bad[key] = value
+        with pytest.raises((AzError, RuntimeError)):
+            q.load_state_dict(bad)
+        assert same_layers(q.layers, kept)
+    q.load_state_dict(good)
+    assert same_layers(q.layers, make(jitter_of(good)).layers)
+
+
+def jitter_of(state):
+    net = Net(h=16)
+    net.load_state_dict(state)
+    return net
