@@ -110,6 +110,7 @@ SIGNATURES = {
     "az_orthogonalize_dev": (C.c_int, [C.c_int, C.c_int, _i64, _i64, _i64, _vp, _vp, C.c_int, _P(_dbl), _dbl, _vp,
                                        C.c_size_t, _vp]),
     "az_muon_step_ws": (C.c_size_t, [_P(az_muon_item), _i64]),
+    "az_muon_step_check": (C.c_int, [C.c_int, _P(az_muon_item), _i64, _dbl, _dbl, _dbl, C.c_int, _P(_dbl), _dbl]),
     "az_muon_step_dev": (C.c_int, [C.c_int, C.c_int, _P(az_muon_item), _i64, _dbl, _dbl, C.c_int, _dbl, C.c_int, _P(_dbl),
                                    _dbl, _vp, C.c_size_t, _vp]),
     "az_set_root_children": (C.c_int, [_vp, _vp, _vp, _vp]),

@@ -951,11 +951,14 @@ size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols) {
     return plan(J, rows, cols, nullptr) * (size_t)(batch < MAX_JOBS ? batch : MAX_JOBS);
 }
 
-static int ortho_check(int dtype, int steps, const double* coeffs, double eps, const void* ws, size_t ws_bytes, size_t need) {
+static int ortho_check(int dtype, int steps, const double* coeffs, double eps) {
     if (!dtype_ok(dtype)) return refuse("az_orthogonalize: unknown dtype");
     if (steps < 1 || steps > 16) return refuse("az_orthogonalize: steps is 1..16");
     if (!(eps > 0) || !isfinite(eps)) return refuse("az_orthogonalize: eps must be positive and finite");
     if (!coeffs_ok(steps, coeffs)) return refuse("az_orthogonalize: these coefficients leave the range of the products");
+    return AZ_OK;
+}
+static int ws_check(const void* ws, size_t ws_bytes, size_t need) {
     if (ws_bytes < need || (need && (!ws || ((uintptr_t)ws & 255))))
         return refuse("az_orthogonalize: workspace too small or not aligned to 256 bytes");
     return AZ_OK;
@@ -965,7 +968,8 @@ int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int
                          int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes, void* stream) {
     if (batch < 0 || batch > (i64)1 << 31 || !dims_ok(rows, cols))
         return refuse("az_orthogonalize: bad shape (rows and cols are 1..32768)");
-    int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_orthogonalize_ws(batch, rows, cols));
+    int rc = ortho_check(dtype, steps, coeffs, eps);
+    if (rc == AZ_OK) rc = ws_check(ws_dev, ws_bytes, az_orthogonalize_ws(batch, rows, cols));
     if (rc != AZ_OK) return rc;
     if (batch > 0 && (!g_dev || !out_dev)) return refuse("az_orthogonalize: null pointer");
     const size_t all = (size_t)batch * rows * cols * dtype_size(dtype);
@@ -1032,9 +1036,8 @@ size_t az_muon_step_ws(const az_muon_item* items, int64_t n) {
     return most;
 }
 
-int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n, double lr, double momentum, int nesterov,
-                     double weight_decay, int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes,
-                     void* stream) {
+int az_muon_step_check(int dtype, const az_muon_item* items, int64_t n, double lr, double momentum, double weight_decay, int steps,
+                       const double* coeffs, double eps) {
     if (n < 0 || n > 65536 || (n > 0 && !items)) return refuse("az_muon_step: bad item list");
     if (!dtype_ok(dtype)) return refuse("az_muon_step: unknown dtype");
     for (int64_t i = 0; i < n; i++) {
@@ -1050,7 +1053,14 @@ int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n
     if (!apart) return refuse("az_muon_step: weights and momenta must not overlap each other or a gradient");
     if (!isfinite(lr) || !isfinite(weight_decay) || !(momentum >= 0 && momentum < 1))
         return refuse("az_muon_step: bad lr, weight_decay or momentum (0 <= momentum < 1)");
-    int rc = ortho_check(dtype, steps, coeffs, eps, ws_dev, ws_bytes, az_muon_step_ws(items, n));
+    return ortho_check(dtype, steps, coeffs, eps);
+}
+
+int az_muon_step_dev(int device, int dtype, const az_muon_item* items, int64_t n, double lr, double momentum, int nesterov,
+                     double weight_decay, int steps, const double* coeffs, double eps, void* ws_dev, size_t ws_bytes,
+                     void* stream) {
+    int rc = az_muon_step_check(dtype, items, n, lr, momentum, weight_decay, steps, coeffs, eps);
+    if (rc == AZ_OK) rc = ws_check(ws_dev, ws_bytes, az_muon_step_ws(items, n));
     if (rc != AZ_OK) return rc;
     DeviceScope dev(device);
     if (dev.rc != AZ_OK || n == 0) return dev.rc;

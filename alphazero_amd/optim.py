@@ -10,6 +10,7 @@ from ._abi import AzError, check, lib
 from ._tensors import DTYPES, no_grad, same_device, stream_of, workspace, written
 
 COEFFS = (3.4445, -4.7750, 2.0315)
+MAX_DIM = 32768   # of a matrix
 
 
 def _coeffs(coeffs):
@@ -44,19 +45,13 @@ def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, out=None):
     return out
 
 
-def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS, eps=1e-7):
-    """One update, in place, of weight matrices by orthogonalised momentum; for each of them
-
-        m <- momentum m + (1 - momentum) g;   u = momentum m + (1 - momentum) g if nesterov else m
-        w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
-
-    weights, grads: lists of contiguous tensors [rows, ...] of one dtype, seen as [rows, rest]; momenta: float32 of the same
-    shapes.  No weight or momentum may overlap another one or a gradient."""
+def _items(weights, grads, momenta):
+    """the tensors of a muon_step call, checked: (device, dtype code, items)"""
     n = len(weights)
     if len(grads) != n or len(momenta) != n:
         raise AzError("muon_step: as many gradients and momenta as weights")
     if n == 0:
-        return
+        return None, None, None
     dt = weights[0].dtype
     if dt not in DTYPES:
         raise AzError("muon_step: weights must be float32, float16 or bfloat16")
@@ -74,18 +69,35 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         it.w_dev, it.g_dev, it.m_dev = w.data_ptr(), g.data_ptr(), m.data_ptr()
         it.rows = rows = w.shape[0]
         it.cols = w.numel() // rows
-    L = lib()
+    return dev, DTYPES[dt], items
+
+
+def _update(dev, code, items, weights, momenta, lr, momentum, nesterov, weight_decay, steps, coeffs, eps):
+    L, n = lib(), len(weights)
     nws = L.az_muon_step_ws(items, n)
     ws, wsp = workspace(nws, weights[0])
-    check(L.az_muon_step_dev(dev, DTYPES[dt], items, n, lr, momentum, 1 if nesterov else 0, weight_decay, steps, _coeffs(coeffs),
+    check(L.az_muon_step_dev(dev, code, items, n, lr, momentum, 1 if nesterov else 0, weight_decay, steps, _coeffs(coeffs),
                              eps, wsp, nws, stream_of(dev)))
     written(*weights, *momenta)
 
 
+def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS, eps=1e-7):
+    """One update, in place, of weight matrices by orthogonalised momentum; for each of them
+
+        m <- momentum m + (1 - momentum) g;   u = momentum m + (1 - momentum) g if nesterov else m
+        w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
+
+    weights, grads: lists of contiguous tensors [rows, ...] of one dtype, seen as [rows, rest]; momenta: float32 of the same
+    shapes.  No weight or momentum may overlap another one or a gradient."""
+    dev, code, items = _items(weights, grads, momenta)
+    if items is not None:
+        _update(dev, code, items, weights, momenta, lr, momentum, nesterov, weight_decay, steps, coeffs, eps)
+
+
 class Muon(torch.optim.Optimizer):
     """torch optimiser around muon_step, for the matrices and convolutions of a network that is trained beside the engine (the
-    reference's Base.train_step calls self.opt, NetworkBase.py:26-62): weights of at least two dimensions, seen as
-    [out, rest].  Biases and norms belong to another optimiser (`matrices_of` tells them apart).  Momenta are float32."""
+    reference's Base.train_step calls self.opt, NetworkBase.py:26-62): weights of at least two dimensions in any memory format, seen as
+    [out, rest], both up to 32768.  Biases and norms belong to another optimiser (`matrices_of` tells them apart).  Momenta are float32."""
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coeffs=COEFFS, eps=1e-7):
         if not lr >= 0.0:
@@ -98,34 +110,46 @@ class Muon(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         for p in self.param_groups[-1]["params"]:
-            if p.dim() < 2 or p.dtype not in DTYPES:
+            if p.dim() < 2 or p.dtype not in DTYPES or max(p.shape[0], p[:1].numel()) > MAX_DIM:
                 del self.param_groups[-1]
-                raise ValueError("Muon takes float32, float16 or bfloat16 weights of at least two dimensions, not %s %s"
-                                 % (tuple(p.shape), p.dtype))
+                raise ValueError("Muon takes float32, float16 or bfloat16 weights of at least two dimensions, [out, rest] up to %d, not %s %s"
+                                 % (MAX_DIM, tuple(p.shape), p.dtype))
 
     @torch.no_grad()
     def step(self, closure=None):
+        """All weights that have a gradient, or, where one is refused, none of them."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        calls = []   # one for the weights of a group, device and dtype
         for group in self.param_groups:
-            lists = {}   # one call for the weights of a device and dtype
+            lists = {}
             for p in group["params"]:
                 if p.grad is None or p.numel() == 0:
                     continue
                 if p.grad.is_sparse:
                     raise AzError("Muon: sparse gradients are not supported")
-                state = self.state[p]
-                if "momentum" not in state:
-                    state["momentum"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
-                w, g, m = lists.setdefault((p.device, p.dtype), ([], [], []))
-                w.append(p.detach())
-                g.append(p.grad.detach().to(p.dtype).contiguous())
-                m.append(state["momentum"])
-            for w, g, m in lists.values():
-                muon_step(w, g, m, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
-                          weight_decay=group["weight_decay"], steps=group["steps"], coeffs=group["coeffs"], eps=group["eps"])
+                m = self.state[p].get("momentum") if p in self.state else None
+                if m is None:
+                    m = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                at = lists.setdefault((p.device, p.dtype), ([], [], [], []))
+                at[0].append(p)
+                at[1].append(p.detach().contiguous())     # itself, but of one in another memory format
+                at[2].append(p.grad.detach().to(p.dtype).contiguous())
+                at[3].append(m)
+            hyper = {k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "coeffs", "eps")}
+            calls += [(at, _items(*at[1:]), hyper) for at in lists.values()]
+        if len(calls) > 1:   # a single call is refused whole by itself
+            for _, (_, code, items), h in calls:
+                check(lib().az_muon_step_check(code, items, len(items), h["lr"], h["momentum"], h["weight_decay"], h["steps"],
+                                               _coeffs(h["coeffs"]), h["eps"]))
+        for (params, weights, _, momenta), (dev, code, items), hyper in calls:
+            _update(dev, code, items, weights, momenta, **hyper)
+            for p, w, m in zip(params, weights, momenta):
+                self.state[p]["momentum"] = m
+                if w.data_ptr() != p.data_ptr():
+                    p.copy_(w)
         return loss
 
     def load_state_dict(self, state_dict):

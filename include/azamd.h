@@ -353,6 +353,10 @@ typedef struct az_muon_item {
     int64_t rows, cols;
 } az_muon_item;
 size_t az_muon_step_ws(const az_muon_item *items, int64_t n);
+/* The checks of az_muon_step_dev but those of its workspace and device, and nothing else: AZ_OK or AZ_ERR_ARG.  For an update of several
+ * calls that is to be made whole or not at all. */
+int az_muon_step_check(int dtype, const az_muon_item *items, int64_t n, double lr, double momentum, double weight_decay, int steps,
+                       const double *coeffs, double eps);
 int az_muon_step_dev(int device, int dtype, const az_muon_item *items, int64_t n, double lr, double momentum, int nesterov,
                      double weight_decay, int steps, const double *coeffs, double eps, void *ws_dev, size_t ws_bytes,
                      void *stream);

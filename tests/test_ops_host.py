@@ -214,3 +214,35 @@ def test_quotients_are_the_exact_ones():
             qd += 1 if 2 * rem > si or (2 * rem == si and qd & 1) else 0
             want.append(max(-127, min(127, qd if v >= 0 else -qd)))
         assert np.array_equal(quant1(x, np.full_like(x, s)), np.array(want))
+
+
+def test_muon_check_alone():
+    """az_muon_step_check: what az_muon_step_dev refuses, without a device and a workspace"""
+    L = _abi.lib()
+
+    def call(items, dtype=0, lr=0.1, momentum=0.9, wd=0.0, steps=5, coeffs=optim.COEFFS, eps=1e-7):
+        arr = (_abi.az_muon_item * max(len(items), 1))()
+        for a, (w, g, m, r, c) in zip(arr, items):
+            a.w_dev, a.g_dev, a.m_dev, a.rows, a.cols = w, g, m, r, c
+        return L.az_muon_step_check(dtype, arr, len(items), lr, momentum, wd, steps, (C.c_double * 3)(*coeffs), eps)
+
+    one, two = (0x1000, 0x2000, 0x3000, 4, 4), (0x4000, 0x5000, 0x6000, 4, 4)
+    assert call([]) == 0 and call([one, two]) == 0
+    _refused(call([one, (0x1020, 0x5000, 0x6000, 4, 4)]), "overlap")
+    _refused(call([(0x1000, 0x2000, 0x3000, 4, 32769)]), "shape")
+    _refused(call([(0x1000, 0, 0x3000, 4, 4)]), "null")
+    _refused(call([one], dtype=3), "dtype")
+    _refused(call([one], lr=float("inf")), "lr")
+    _refused(call([one], momentum=-0.1), "momentum")
+    _refused(call([one], steps=0), "steps")
+    _refused(call([one], eps=0.0), "eps")
+    _refused(call([one], coeffs=(9.0, 0.0, 0.0)), "coefficients")
+
+
+def test_a_refused_muon_step_leaves_no_state():
+    a, b = [torch.nn.Parameter(torch.randn(3, 4)) for _ in range(2)]
+    opt = optim.Muon([{"params": [a]}, {"params": [b]}])
+    a.grad, b.grad = torch.ones(3, 4), torch.ones(3, 4)
+    with pytest.raises(_abi.AzError, match="GPU"):
+        opt.step()
+    assert not opt.state
