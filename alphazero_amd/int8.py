@@ -62,7 +62,6 @@ def _layer(what, m, k, w, w_scale, bias, residual, act, dtype, out):
     if out is None:
         out, ld_y = torch.empty((m, n), dtype=dtype, device=w.device), n
     else:
-        written(out)
         o_m, o_n, ld_y = rows_of(out, what, "out")
         if out.dtype is not dtype or o_m != m or o_n != n:
             raise AzError("%s: out must be [%d, %d] of the output's dtype" % (what, m, n))
@@ -77,14 +76,17 @@ def matmul(q, scale, w, w_scale, bias=None, residual=None, act="none", dtype=tor
     if q.dtype is not torch.int8:
         raise AzError("matmul: q must be int8")
     m, k, ld_q = rows_of(q, "matmul", "q")
-    no_grad("matmul", scale, w_scale, bias, residual)
+    no_grad("matmul", scale, w_scale, bias, residual, out)
     dev = same_device("matmul", q, scale, w, w_scale, bias, residual, out)
     s = vector(scale, m, "matmul", "scale")
+    given = out is not None
     n, wp, ld_w, out, tail = _layer("matmul", m, k, w, w_scale, bias, residual, act, dtype, out)
     L, qp = lib(), q.data_ptr()
     nws = L.az_i8_matmul_ws(m, n, k, qp, ld_q, wp, ld_w)
     ws, wsp = workspace(nws, q)
     check(L.az_i8_matmul_dev(dev, m, n, k, qp, ld_q, s, wp, ld_w, *tail, wsp, nws, stream_of(dev)))
+    if given:
+        written(out)
     return out
 
 
@@ -93,11 +95,14 @@ def linear(x, w, w_scale, bias=None, residual=None, act="none", out=None):
     if x.dtype not in DTYPES:
         raise AzError("linear: x must be float32, float16 or bfloat16")
     m, k, ld_x = rows_of(x, "linear", "x")
-    no_grad("linear", x, w_scale, bias, residual)
+    no_grad("linear", x, w_scale, bias, residual, out)
     dev = same_device("linear", x, w, w_scale, bias, residual, out)
+    given = out is not None
     n, wp, ld_w, out, tail = _layer("linear", m, k, w, w_scale, bias, residual, act, x.dtype, out)
     L, xp = lib(), x.data_ptr()
     nws = L.az_i8_linear_ws(m, n, k, wp, ld_w)
     ws, wsp = workspace(nws, x)
     check(L.az_i8_linear_dev(dev, m, n, k, xp, ld_x, wp, ld_w, *tail, wsp, nws, stream_of(dev)))
+    if given:
+        written(out)
     return out

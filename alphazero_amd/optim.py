@@ -25,7 +25,7 @@ def orthogonalize(g, steps=5, coeffs=COEFFS, eps=1e-7, out=None):
     Values of X are held to 2^-39 at best: of a matrix whose norm is 10^-4 of eps or less, fewer bits than float32's remain."""
     if g.dtype not in DTYPES or g.dim() < 2:
         raise AzError("orthogonalize: g must be float32, float16 or bfloat16 of at least two dimensions")
-    no_grad("orthogonalize", g)
+    no_grad("orthogonalize", g, out)
     dev = same_device("orthogonalize", g, out)
     rows, cols = g.shape[-2:]
     if out is None:

@@ -246,3 +246,15 @@ def test_a_refused_muon_step_leaves_no_state():
     with pytest.raises(_abi.AzError, match="GPU"):
         opt.step()
     assert not opt.state
+
+
+def test_outputs_that_autograd_follows_are_refused():
+    """written by a kernel, they would keep the graph of what they held before"""
+    w, s = torch.zeros(6, 8, dtype=torch.int8), torch.ones(6)
+    for out in (torch.zeros(6, 6, requires_grad=True), torch.zeros(6, 6, requires_grad=True) * 2):
+        for call in (lambda: int8.matmul(w, s, w, s, out=out), lambda: int8.linear(torch.zeros(6, 8), w, s, out=out),
+                     lambda: optim.orthogonalize(torch.zeros(6, 6), out=out)):
+            with pytest.raises(_abi.AzError, match="no backward"):
+                call()
+            with torch.no_grad(), pytest.raises(_abi.AzError, match="GPU"):
+                call()
