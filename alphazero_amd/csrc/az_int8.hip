@@ -167,7 +167,9 @@ __device__ inline u32 lanes_max(u32 v) {
 // magnitude and its integers.  FAST: the columns are whole pieces, rows are 16-byte aligned, offsets fit 31 bits and the factors
 // of a row's offset 24 (full-rate multiplications); rows that are not there are read behind the end of the buffer, as zeros.
 // 86016 rows of 9 x 128 fp16 (22 MB read, 99 MB written): 37 us, 3.3 TB/s of the 5.1 that a copy reaches; what bounds it is the VALU
-// (40 instructions for 8 values: the quotient, how near a half it is, the packing) beside two trips to memory, index and rows.  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
+// (94 instructions for 8 values: the quotient, how near a half it is, the packing, the largest: 18.2 M a wave, of 4 cycles each, on 1024
+// SIMDs are the kernel's 69 k cycles).  The same in bf16 43 us (conversions), in float32 85 (288 pieces, a row to 256 lanes: see
+// rows_dispatch).  4099 x 1001 float32: 6.1 us, 3.4 TB/s.
 // One row of 4096 bf16: 3.6 us, all of it latency: the load, the reduction over 4 waves, the launch.
 template <class T, int LANES, int NP, bool FAST>
 __global__ __launch_bounds__(256) void k_i8_quantize(Rows R) {
@@ -367,11 +369,12 @@ __device__ inline void put(const Mm& p, i64 m, i64 n, int sum, float scale) {
 
 // Rows of both operands at multiples of 16 bytes, k a multiple of 16.  blockIdx.y: which of the `splits` parts of k (whole
 // steps each); with more than one the int32 sums go to part[split][m][n] and k_i8_join adds them.
-// 8192^3, 256 x 256 tiles: 545 us, 2.0 POP/s of the 2.5 that the library's product reaches; the matrix pipe is busy for 59 % at
-// 1.66 GHz (power): a k slice costs as many LDS cycles as MFMA cycles.  86016 x 128 x 1152, 128 x 128 tiles: 29 us, 4.2 TB/s of rows
-// read and results written, SiLU on the way.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 7.8 us, one after the other:
+// 8192^3, 256 x 256 tiles: 504 us, 2.2 POP/s of the 2.44 that the library's product reaches; of 804 k cycles the matrix pipe is busy for
+// 65 %, LDS for 25 %; a CU's two waves a SIMD spend 30 % at loads and barriers.  86016 x 128 x 1152, 128 x 128 tiles: 27.5 us, 4.4 TB/s of rows
+// read and results written, SiLU on the way.  777 x 1003 x 1031, 64 x 64 tiles, 208 workgroups: 7.5 us, one after the other:
 // launch, first tiles, 17 steps, residual, stores.
-// RES: with a residual, whose values take registers (128 x 128 tile: 96, 70 without: three workgroups a CU).
+// RES: with a residual, whose values take registers (128 x 128 tile: 96, and 70 without, with which three workgroups a CU fit and not
+// two: 86016 x 128 x 1152 29.2 us with one form for both, 27.5 with two; 8192^3 541 and 504).
 template <class T, class S, bool RES>
 __global__ __launch_bounds__(S::THREADS) void k_i8_mm_tile(Mm p, u32 tiles_m, u32 tiles_n, u32 steps_per_split, int* part) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
@@ -665,7 +668,7 @@ static bool few_rows(i64 m, i64 n, i64 k, bool aligned) {
 constexpr i64 TILE_MAX_LD = 1 << 22;  // row distance up to which a tile's addresses fit 32 bits
 
 using Tile256 = TileShape<256, 256, 2, 4, 4, 1>;   // 128 KB; 128 x 64 a wave: 6 operand reads for 8 MFMAs
-using Tile128 = TileShape<128, 128, 4, 2, 3, 1>;   // 48 KB: three workgroups a CU, whose stores run under each other's loads
+using Tile128 = TileShape<128, 128, 4, 2, 3, 1>;   // 48 KB: three workgroups a CU (two with a residual), whose stores run under each other's loads
 using Tile64 = TileShape<64, 64, 2, 2, 3, 2>;      // few tiles: what counts is the way from step to step, so a barrier every two
 
 // How a product is computed; a function of the sizes and alignments alone, so that the workspace can be asked for first.
@@ -770,7 +773,9 @@ static void rows_go(const Rows& R, hipStream_t st) {
     k_i8_quantize<T, LANES, NP, FAST><<<dim3((u32)(b < 1 << 20 ? b : 1 << 20)), dim3(256), 0, st>>>(R);
 }
 // Few lanes to a row waste the fewest on its end and on its reduction; with few rows it takes more lanes to fill the chip (us, 16 lanes
-// | 64: 300 fp16 values, 16384 rows 8.1 | 10.0, 8192 rows 7.3 | 6.7; 1152 values, 65536 rows 41.3 | 42.8, 16384 rows 17.3 | 15.1).
+// | 64: 300 fp16 values, 16384 rows 8.1 | 10.0, 8192 rows 7.3 | 6.7; 1152 values, 65536 rows 41.3 | 42.8, 16384 rows 17.3 | 15.1).  Longer
+// rows than the forms' 144 and 256 pieces go to 256 lanes, whose reduction takes two barriers (86016 rows of 1152 float32, 288 pieces:
+// 85 us for a floor of 29; no form between has been tried).
 template <class T, bool FAST>
 static void rows_dispatch(const Rows& R, hipStream_t st) {
     const u32 P = R.pieces;

@@ -227,10 +227,11 @@ struct Staged {
 };
 
 // 2048 x 2048: Gram 46 us (0.56 PFLOP/s of fp16 products, the lower triangle's counted), polynomial 48, step 57 (0.90), last 54; a
-// library's fp16 product reaches 1.38 at 8192^3, this one 1.03 over whole calls at 4096 x 4096.  Two thirds are the loop, bound
-// by LDS (operand reads, the loads' writes), the rest the launch, the first tiles and 16-32 MB of stores that all workgroups make at
-// once.  272 symmetric tiles on 256 CUs cost 12 us more than 240 (1920 x 1920: 36), but 64 x 64 tiles, longer and shorter rings and 8
-// waves each came out between 0 and 20 % slower over the whole call.  384 x 384 of two matrices: 7.6 us, latency.
+// library's fp16 product reaches 1.38 at 8192^3, this one 1.03 over whole calls at 4096 x 4096.  Neither pipe is full: of the Gram launch's
+// cycles the matrix pipe works in 37 %, of a step's in 55 %, LDS in 20 %.  272 or 256 tiles on 256 CUs leave one wave a SIMD on most of them,
+// which no other covers while it waits: 22 % of its cycles at loads and barriers (one a step), 32 % for the pipe it needs next.  272 symmetric
+// tiles cost 12 us more than 240 (1920 x 1920: 36), but 64 x 64 tiles, longer and shorter rings and 8 waves each came out between 0 and
+// 20 % slower over the whole call.  384 x 384 of two matrices: 7.6 us, latency.
 template <int MODE, class S, class T>
 __global__ __launch_bounds__(S::THREADS) void k_ortho_product(Jobs js, Hyper h, int cur, Op op) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
@@ -523,6 +524,7 @@ __global__ __launch_bounds__(256) void k_narrow_sum(Jobs js) {
 struct Narrow {
     float p_unit, x_unit;
 };
+// 128 registers a wave (16 of them share a CU) are not enough: the compiler keeps 28 to 48 bytes a lane in scratch, by the form.
 template <class T, bool LASTSTEP, bool TWO>
 __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int cur, Narrow pass) {
     extern __shared__ __attribute__((aligned(128))) u8 lds[];
@@ -614,7 +616,7 @@ __global__ __launch_bounds__(NTHREADS) void k_narrow_step(Jobs js, Hyper h, int 
         times(bufA, bufB, bufA, 0x1p-11f, false);
         times(bufA, bufB, bufA, 0x1p-11f, false);
         times(bufA, bufA, bufA, 0x1p-24f, true);
-        fetch(first);   // not earlier: its 32 registers spill others
+        fetch(first);   // not earlier: its 32 registers would spill more
         times(bufA, bufB, bufB, pass.p_unit, false);
     }
     // 3. the panels

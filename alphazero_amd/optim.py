@@ -1,5 +1,6 @@
 """Orthogonalised updates of weight matrices (csrc/az_ortho.hip; include/azamd.h: az_orthogonalize_dev, az_muon_step_dev), for
-the training step between ReplayBuffer.dataloader and CNN.sync_from.
+the training step between ReplayBuffer.dataloader and CNN.sync_from.  The method, momentum orthogonalised by a quintic Newton-Schulz
+iteration with these coefficients, was published as Muon (K. Jordan and others, 2024).
 """
 import ctypes as C
 
