@@ -49,7 +49,8 @@ def planes_to_packed(state):
 class CNN:
     def __init__(self, lr=0, in_dim=3, h_dim=128, out_dim=7, device="cuda"):
         if (in_dim, h_dim, out_dim) != (3, 128, 7):
-            raise _abi.AzError("the fused kernel implements the reference architecture only: in_dim=3, h_dim=128, out_dim=7")
+            raise _abi.AzError("the fused kernel implements the reference architecture only: in_dim=3, h_dim=128, out_dim=7; "
+                               "alphazero_amd.int8_net.Int8CNN evaluates trained networks of other widths and boards")
         self.lr = lr
         self.device = device
         self.n_actions = out_dim
