@@ -16,10 +16,13 @@ from . import int8
 from ._abi import AzError
 
 BN_EPS = 1e-5   # torch.nn.BatchNorm2d's
+F32_MAX = torch.finfo(torch.float32).max
 LOCK = threading.RLock()   # held while a network's tensors on the device change
 
 
 def capturing(device):
+    if torch.cuda.current_device() == device.index:      # as a rule; making it current takes 5 us
+        return torch.cuda.is_current_stream_capturing()
     with torch.cuda.device(device):
         return torch.cuda.is_current_stream_capturing()
 
@@ -131,12 +134,12 @@ class Int8CNN:
             w, bias = out[name]
             if w.shape[1] != inputs * taps or (outputs is not None and w.shape[0] != outputs) or bias.shape != (w.shape[0],):
                 raise AzError("Int8CNN: %s does not fit the layers around it" % name)
-            if not (torch.isfinite(w.float()).all() and torch.isfinite(bias.float()).all()):
+            if not all(-F32_MAX <= lo and hi <= F32_MAX for lo, hi in (w.aminmax(), bias.aminmax())):      # nor a NaN, which is no bound
                 raise AzError("Int8CNN: %s is not finite in float32 once its BatchNorm is folded in" % name)
             return w.shape[0]
 
         out = {"stem": folded("hidden.0", "hidden.1")}
-        h = fits("stem", get("hidden.0.weight").shape[1], 9)
+        h = fits("stem", sd["hidden.0.weight"].shape[1], 9)
         blocks = sorted({int(m.group(1)) for m in (re.match(r"hidden\.(\d+)\.conv\.0\.weight$", k) for k in sd) if m})
         for i, b in enumerate(blocks):
             out["conv%d" % i] = folded("hidden.%d.conv.0" % b, "hidden.%d.conv.1" % b)
@@ -176,8 +179,8 @@ class Int8CNN:
             self._tables += (t,)
         return t[:rows]
 
-    def _conv3(self, x, name, boards):
-        q, s = int8.quantize_rows(x, index=self._neighbours(boards))
+    def _conv3(self, x, name, table):
+        q, s = int8.quantize_rows(x, index=table)
         w, ws, b = self.layers[name]
         return int8.matmul(q, s, w, ws, bias=b, act="silu", dtype=self.dtype)
 
@@ -199,9 +202,10 @@ class Int8CNN:
                 return (torch.empty(0, self.n_actions, device=self.device), torch.empty(0, self.layers["value_out"][0].shape[0], device=self.device))
             self._captured = self._captured or capturing(self.device)
             x = planes.to(self.device, self.dtype).permute(0, 2, 3, 1).reshape(B * self.cells, self.in_dim).contiguous()
-            x = self._conv3(x, "stem", B)
+            table = self._neighbours(B)
+            x = self._conv3(x, "stem", table)
             for i in range(self.n_blocks):
-                t = self._conv3(x, "conv%d" % i, B)
+                t = self._conv3(x, "conv%d" % i, table)
                 w, ws, b = self.layers["mix%d" % i]
                 x = int8.linear(t, w, ws, bias=b, residual=x, act="silu")
             return self._logits(x, "policy", B), self._logits(x, "value", B)

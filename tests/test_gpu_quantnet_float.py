@@ -51,7 +51,7 @@ def test_layers_are_the_modules(in_dim, h, out_dim, board, boards):
     def conv3(name, conv, bn, act):
         c = net.get_submodule(conv)
         x = seen[conv][0]
-        y = q._conv3(gpu(rows_of(x)), name, boards)
+        y = q._conv3(gpu(rows_of(x)), name, q._neighbours(boards))
         rows = torch.nn.functional.unfold(x, 3, padding=1).transpose(1, 2).reshape(boards * board[0] * board[1], -1)
         b = net.get_submodule(bn).bias.detach().abs() + (net.get_submodule(bn).running_mean * factor(bn)).abs()
         check(y, rows_of(seen[act][1]), rows, c.weight.detach().reshape(c.weight.shape[0], -1), factor(bn), name, b)
