@@ -89,7 +89,8 @@ def muon_step(weights, grads, momenta, lr, momentum=0.95, nesterov=True, weight_
         w <- (1 - lr weight_decay) w - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
     weights, grads: lists of contiguous tensors [rows, ...] of one dtype, seen as [rows, rest]; momenta: float32 of the same
-    shapes.  No weight or momentum may overlap another one or a gradient."""
+    shapes.  No weight or momentum may overlap another one or a gradient.  Float32 weights come out the same, bit for bit, whatever else
+    is in the lists; 16-bit ones may differ in their last bits (several steps at once, where the lists as a whole gain by it)."""
     dev, code, items = _items(weights, grads, momenta)
     if items is not None:
         _update(dev, code, items, weights, momenta, lr, momentum, nesterov, weight_decay, steps, coeffs, eps)

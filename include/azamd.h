@@ -330,14 +330,15 @@ int az_i8_linear_dev(int device, int64_t m, int64_t n, int64_t k, const void *x_
 
 /* Orthogonalisation of `batch` matrices [rows][cols] (contiguous) by Newton-Schulz products: X = G / (||G||_F + eps), then
  * `steps` times X <- a X + (b A + c A^2) X with A = X X^T (on the shorter side), coeffs = {a, b, c}.  Products are
- * float32-accurate (fp16 matrix pipe, operands split into two halves): values of X are off by 2^-23 of themselves, below 2^-16 by 2^-39.  What a
- * norm far below eps leaves of X loses relative accuracy by that, and only that (1024 x 1024, relative error at eps / ||G|| of 100, 10^4,
- * 10^6: 8e-7, 1e-5, 1e-3).  out may be g itself.  steps 1..16, eps > 0.  Coefficients whose
+ * float32-accurate (fp16 matrix pipe, operands split into two halves): values of X are off by 2^-23 of themselves, below 2^-16 by
+ * 2^-39.  What a norm far below eps leaves of X loses relative accuracy by that, and only that (1024 x 1024, relative error at
+ * eps / ||G|| of 100, 10^4, 10^6: 8e-7, 1e-5, 1e-3).  out may be g itself.  steps 1..16, eps > 0.  Coefficients whose
  * iteration takes a singular value of [0, 1] above 2, or b A + c A^2 + a out of [-16, 16], are AZ_ERR_ARG (the halves' range).
  * A matrix that holds a NaN or an infinity comes out as NaN.  rows, cols <= 32768.
- * In float32 the steps are made one after the other, and a matrix comes out the same, bit for bit, beside any others.  Where the result has 16 bits several may be made at once, on the s x s products
- * alone, when that is faster for the matrices of the call together: a matrix's result can then differ in its last bits (float32
- * errors of up to 5e-6 instead of 2e-6, before the rounding) from the one it has alone. */
+ * In float32 the steps are made one after the other, and a matrix comes out the same, bit for bit, beside any others.  Where the
+ * result has 16 bits several may be made at once, on the s x s products alone, when that is faster for the matrices of the call
+ * together: a matrix's result can then differ in its last bits (float32 errors of up to 5e-6 instead of 2e-6, before the rounding)
+ * from the one it has alone. */
 size_t az_orthogonalize_ws(int64_t batch, int64_t rows, int64_t cols);
 int az_orthogonalize_dev(int device, int dtype, int64_t batch, int64_t rows, int64_t cols, const void *g_dev, void *out_dev,
                          int steps, const double *coeffs, double eps, void *ws_dev, size_t ws_bytes, void *stream);
